@@ -18,6 +18,9 @@
 
 use core::ffi::{c_char, c_void};
 
+/// The operators around the linear (`include/qmm_block.h`).
+pub mod block;
+
 pub const QMM_ABI_VERSION: i32 = 2;
 
 /// Status codes (replace the `candle_core::Error` results of quant.rs).

@@ -14,6 +14,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -42,7 +43,7 @@ def sources() -> list[str]:
 
 def headers() -> list[str]:
     return (sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + sorted(glob.glob(os.path.join(CSRC, "*.h")))
-            + [os.path.join(ROOT, "include", "qmm.h")])
+            + sorted(glob.glob(os.path.join(ROOT, "include", "*.h"))))
 
 
 def is_stale() -> bool:
@@ -58,13 +59,18 @@ def build(verbose: bool = False, force: bool = False) -> str:
         return LIB
     os.makedirs(OUT_DIR, exist_ok=True)
     nvcc = nvcc_path()
-    objs = []
-    for src in sources():
+
+    def compile_one(src: str):
         obj = os.path.join(OUT_DIR, os.path.basename(src)[:-3] + ".o")
         cmd = [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, "-c", src, "-o", obj]
         if verbose:
             cmd += ["-Xptxas", "-v"]
-        res = subprocess.run(cmd, capture_output=True, text=True)
+        return src, obj, subprocess.run(cmd, capture_output=True, text=True)
+
+    objs = []
+    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        results = list(pool.map(compile_one, sources()))
+    for src, obj, res in results:
         if verbose or res.returncode != 0:
             sys.stderr.write(res.stdout + res.stderr)
         if res.returncode != 0:

@@ -92,8 +92,19 @@ bool gemv_pdl_enabled() {
     return on;
 }
 
+qmm_status check_device() {
+    int dev = -1;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_fail(e, "no CUDA device");
+    int major = 0;
+    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+    if (major != 10) return fail(QMM_ERR_CUDA, "device %d is not sm_100 (compute capability %d.x)", dev, major);
+    return QMM_OK;
+}
+
 }  // namespace qmm
 
+using qmm::check_device;
 using qmm::fail;
 
 // An empty kernel whose attributes report the architecture the library's
@@ -106,16 +117,6 @@ static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 
 static bool valid_activation(int32_t a) {
     const int32_t act = a & 0xFF;
     return (a & ~(0xFF | QMM_EPILOGUE_RESIDUAL_MUL)) == 0 && act >= QMM_ACT_NONE && act <= QMM_ACT_SILU;
-}
-
-static qmm_status check_device() {
-    int dev = -1;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return qmm::cuda_fail(e, "no CUDA device");
-    int major = 0;
-    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-    if (major != 10) return fail(QMM_ERR_CUDA, "device %d is not sm_100 (compute capability %d.x)", dev, major);
-    return QMM_OK;
 }
 
 extern "C" {

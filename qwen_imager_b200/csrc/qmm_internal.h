@@ -20,6 +20,9 @@ uint32_t *device_error_word();
 // Streaming multiprocessors of the current device.
 int sm_count();
 
+// QMM_OK when the current device is an sm_100 GPU.
+qmm_status check_device();
+
 // Counts kernel launches (exported through qmm_launch_count()).
 void count_launch(uint64_t n = 1);
 
@@ -62,5 +65,9 @@ int gemm_recommended_splits(const qmm_weight &w, int64_t m);
 // f16: x is fp16 and the weights are dequantized to fp16 (QMM_PATH_GEMM_F16).
 qmm_status launch_gemm(const qmm_weight &w, const uint16_t *x, int64_t m, const qmm_epilogue &ep,
                        uint16_t *y, bool pair, int splits, float *ws, cudaStream_t st, bool f16 = false);
+
+// x [rows, k] (element type `elem`, row stride in elements) to MXFP4 (qmm_mx4_quantize).
+qmm_status launch_mx4_quantize(const void *x, int32_t elem, int64_t rows, int64_t k, int64_t row_stride, uint8_t *codes,
+                               uint8_t *scales, cudaStream_t st);
 
 }  // namespace qmm

@@ -1,0 +1,384 @@
+// RMSNorm per head of q and k, and rotary positions with several axes
+// (qmm_qk_norm_rotary).
+//
+// HBM-bound: q and k are read and written once; positions are a few bytes a
+// token.  A warp takes a token and a run of its heads.  Each lane holds the same
+// four pairs of every head (as two runs of four columns), so the token's sines
+// and cosines are computed once per lane and stay in registers over the heads; a
+// head of 8 U columns takes U lanes, 32 / U heads go at a time.
+//
+// The angle is positions * turns in turns.  With turns = f + g (leading and
+// trailing term), p = fl(pos f) and e = pos f - p exact by one fma, the fraction
+// of p is exact and the angle's error stays near 2^-24 turns at any position.
+#include "qmm_internal.h"
+#include "qmm_mx4.cuh"
+
+namespace qmm {
+namespace rotary {
+
+constexpr int kWarps = 4;
+constexpr int kAhead = 4;  // heads in flight per lane group
+
+__device__ __forceinline__ float position_of(const qmm_rotary_args &a, int64_t batch, int64_t token, int axis) {
+    const int64_t i = batch * a.pos_batch_stride + token * a.axes + axis;
+    if (a.pos_kind == 0) return (float)static_cast<const int32_t *>(a.positions)[i];
+    if (a.pos_kind == 1) return (float)static_cast<const int64_t *>(a.positions)[i];
+    return static_cast<const float *>(a.positions)[i];
+}
+
+__device__ __forceinline__ void pair_turn(const qmm_rotary_args &a, int64_t batch, int64_t token, int pair, float *c, float *s) {
+    const float pos = position_of(a, batch, token, a.axis[pair]);
+    const float f = a.turns[2 * pair], g = a.turns[2 * pair + 1];
+    const float p = pos * f;
+    const float e = fmaf(pos, f, -p);
+    const float t = (p - rintf(p)) + fmaf(pos, g, e);
+    sincospif(2.0f * t, s, c);
+}
+
+// Four elements at an address aligned to four elements.
+template <typename T>
+struct Vec4 {
+    uint32_t w[sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ Vec4<T> load_vec4(const T *p) {
+    Vec4<T> r;
+    if constexpr (sizeof(T) == 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        r.w[0] = v.x, r.w[1] = v.y;
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void vec4_to_f32(const Vec4<T> &r, float (&v)[4]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r.w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 f = unpack2<T>(r.w[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_vec4(T *p, const float (&v)[4]) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    }
+}
+
+// G: lanes a head (a power of two, at least dim / 8).  Needs dim % 8 == 0, with
+// halves pairs % 4 == 0, and every head at an address aligned to four elements.
+template <typename T, int G>
+__global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const qmm_rotary_args a, const int heads_per_warp) {
+    constexpr int H = 32 / G;  // heads at a time
+    const int lane = threadIdx.x & 31, u = lane % G, sub = lane / G;
+    const int splits = (a.q_heads + a.k_heads + heads_per_warp - 1) / heads_per_warp;
+    const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int64_t row = unit / splits;
+    if (row >= a.batch * a.tokens) return;
+    const int64_t batch = row / a.tokens, token = row % a.tokens;
+    const int heads = a.q_heads + a.k_heads;
+    const int h0 = (int)(unit % splits) * heads_per_warp, h1 = min(h0 + heads_per_warp, heads);
+    const bool live = u * 8 < a.dim;
+    // This lane's columns: [ca, ca + 4) and [cb, cb + 4), and their pairs.
+    int ca = u * 8, cb = u * 8 + 4, pair = u * 4;
+    if (!a.adjacent && u * 4 < a.pairs) ca = u * 4, cb = a.pairs + u * 4;
+    float cs[4], sn[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        cs[i] = 1.0f, sn[i] = 0.0f;
+        if (pair + i < a.pairs) pair_turn(a, batch, token, pair + i, &cs[i], &sn[i]);
+    }
+    const float inv_dim = 1.0f / (float)a.dim;
+    for (int hb = h0; hb < h1; hb += H * kAhead) {
+        Vec4<T> ra[kAhead], rb[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int h = hb + j * H + sub;
+            ra[j] = Vec4<T>{}, rb[j] = Vec4<T>{};
+            if (h < h1 && live) {
+                const bool isq = h < a.q_heads;
+                const T *src = isq ? static_cast<const T *>(a.q) + batch * a.q_stride[0] + token * a.q_stride[1] + h * a.q_stride[2]
+                                   : static_cast<const T *>(a.k) + batch * a.k_stride[0] + token * a.k_stride[1] +
+                                         (h - a.q_heads) * a.k_stride[2];
+                ra[j] = load_vec4(src + ca);
+                rb[j] = load_vec4(src + cb);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int h = hb + j * H + sub;
+            const bool isq = h < a.q_heads;
+            float va[4], vb[4];
+            vec4_to_f32(ra[j], va);
+            vec4_to_f32(rb[j], vb);
+            const T *w = static_cast<const T *>(isq ? a.q_weight : a.k_weight);
+            if (a.q_weight || a.k_weight) {  // (the shuffles below take the whole warp)
+                float s = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s = fmaf(va[i], va[i], fmaf(vb[i], vb[i], s));
+#pragma unroll
+                for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+                if (w && live) {
+                    const float r = rsqrtf(s * inv_dim + a.eps);
+                    float wa[4], wb[4];
+                    vec4_to_f32(load_vec4(w + ca), wa);
+                    vec4_to_f32(load_vec4(w + cb), wb);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) va[i] *= r * wa[i], vb[i] *= r * wb[i];
+                }
+            }
+            if (h < h1 && live) {
+                float oa[4], ob[4];
+                if (a.adjacent) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        oa[2 * i] = va[2 * i] * cs[i] - va[2 * i + 1] * sn[i];
+                        oa[2 * i + 1] = va[2 * i] * sn[i] + va[2 * i + 1] * cs[i];
+                        ob[2 * i] = vb[2 * i] * cs[i + 2] - vb[2 * i + 1] * sn[i + 2];
+                        ob[2 * i + 1] = vb[2 * i] * sn[i + 2] + vb[2 * i + 1] * cs[i + 2];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        oa[i] = va[i] * cs[i] - vb[i] * sn[i];
+                        ob[i] = va[i] * sn[i] + vb[i] * cs[i];
+                    }
+                }
+                T *dst = isq ? static_cast<T *>(a.q_out) + batch * a.q_out_stride[0] + token * a.q_out_stride[1] + h * a.q_out_stride[2]
+                             : static_cast<T *>(a.k_out) + batch * a.k_out_stride[0] + token * a.k_out_stride[1] +
+                                   (h - a.q_heads) * a.k_out_stride[2];
+                store_vec4(dst + ca, oa);
+                store_vec4(dst + cb, ob);
+            }
+        }
+    }
+}
+
+// Any dim up to 256, any pairs, any alignment: lane l takes pairs l, l + 32, ...
+// and the unrotated columns likewise, element by element.
+template <typename T>
+__global__ void __launch_bounds__(kWarps * 32) rotary_any_kernel(const qmm_rotary_args a, const int heads_per_warp) {
+    const int lane = threadIdx.x & 31;
+    const int splits = (a.q_heads + a.k_heads + heads_per_warp - 1) / heads_per_warp;
+    const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int64_t row = unit / splits;
+    if (row >= a.batch * a.tokens) return;
+    const int64_t batch = row / a.tokens, token = row % a.tokens;
+    const int heads = a.q_heads + a.k_heads;
+    const int h0 = (int)(unit % splits) * heads_per_warp, h1 = min(h0 + heads_per_warp, heads);
+    float cs[4], sn[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        cs[j] = 1.0f, sn[j] = 0.0f;
+        if (lane + 32 * j < a.pairs) pair_turn(a, batch, token, lane + 32 * j, &cs[j], &sn[j]);
+    }
+    const float inv_dim = 1.0f / (float)a.dim;
+    for (int h = h0; h < h1; ++h) {
+        const bool isq = h < a.q_heads;
+        const int hh = isq ? h : h - a.q_heads;
+        const T *src = isq ? static_cast<const T *>(a.q) + batch * a.q_stride[0] + token * a.q_stride[1] + hh * a.q_stride[2]
+                           : static_cast<const T *>(a.k) + batch * a.k_stride[0] + token * a.k_stride[1] + hh * a.k_stride[2];
+        T *dst = isq ? static_cast<T *>(a.q_out) + batch * a.q_out_stride[0] + token * a.q_out_stride[1] + hh * a.q_out_stride[2]
+                     : static_cast<T *>(a.k_out) + batch * a.k_out_stride[0] + token * a.k_out_stride[1] + hh * a.k_out_stride[2];
+        const T *w = static_cast<const T *>(isq ? a.q_weight : a.k_weight);
+        float va[4], vb[4], rest[8];
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int p = lane + 32 * j;
+            va[j] = vb[j] = 0.0f;
+            if (p < a.pairs) {
+                va[j] = elem_to_f32(src[a.adjacent ? 2 * p : p]);
+                vb[j] = elem_to_f32(src[a.adjacent ? 2 * p + 1 : a.pairs + p]);
+            }
+            s = fmaf(va[j], va[j], fmaf(vb[j], vb[j], s));
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = 2 * a.pairs + lane + 32 * j;
+            rest[j] = c < a.dim ? elem_to_f32(src[c]) : 0.0f;
+            s = fmaf(rest[j], rest[j], s);
+        }
+        float r = 1.0f;
+        if (w) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            r = rsqrtf(s * inv_dim + a.eps);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int p = lane + 32 * j;
+            if (p < a.pairs) {
+                const int ia = a.adjacent ? 2 * p : p, ib = a.adjacent ? 2 * p + 1 : a.pairs + p;
+                const float x = w ? va[j] * (r * elem_to_f32(w[ia])) : va[j], y = w ? vb[j] * (r * elem_to_f32(w[ib])) : vb[j];
+                dst[ia] = elem_from_f32<T>(x * cs[j] - y * sn[j]);
+                dst[ib] = elem_from_f32<T>(x * sn[j] + y * cs[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int c = 2 * a.pairs + lane + 32 * j;
+            if (c < a.dim) dst[c] = elem_from_f32<T>(w ? rest[j] * (r * elem_to_f32(w[c])) : rest[j]);
+        }
+        __syncwarp();
+    }
+}
+
+template <typename T>
+static qmm_status launch(const qmm_rotary_args &a, bool fast, cudaStream_t st) {
+    const int heads = a.q_heads + a.k_heads;
+    int g = 4;
+    while (g * 8 < a.dim) g *= 2;
+    const int at_a_time = fast ? 32 / g : 1;
+    // Heads a warp: all of a token's where the tokens alone fill the machine, so
+    // that its sines are computed once; fewer where they do not, down to the
+    // heads that a warp handles at a time.
+    const int64_t rows = a.batch * a.tokens;
+    int64_t splits = 1;
+    const int64_t most = (heads + at_a_time - 1) / at_a_time;
+    while (splits < most && rows * splits < (int64_t)sm_count() * 16) splits *= 2;
+    if (splits > most) splits = most;
+    int per = (int)((heads + splits - 1) / splits);
+    per = (per + at_a_time - 1) / at_a_time * at_a_time;
+    splits = (heads + per - 1) / per;
+    const int64_t blocks = (rows * splits + kWarps - 1) / kWarps;
+    if (blocks > INT32_MAX) return fail(QMM_ERR_UNSUPPORTED, "rotary: %lld tokens are past the launch limits", (long long)rows);
+    const unsigned grid = (unsigned)blocks;
+    if (!fast) rotary_any_kernel<T><<<grid, kWarps * 32, 0, st>>>(a, per);
+    else if (g == 4) rotary_kernel<T, 4><<<grid, kWarps * 32, 0, st>>>(a, per);
+    else if (g == 8) rotary_kernel<T, 8><<<grid, kWarps * 32, 0, st>>>(a, per);
+    else if (g == 16) rotary_kernel<T, 16><<<grid, kWarps * 32, 0, st>>>(a, per);
+    else rotary_kernel<T, 32><<<grid, kWarps * 32, 0, st>>>(a, per);
+    count_launch();
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? QMM_OK : cuda_fail(e, "rotary launch");
+}
+
+}  // namespace rotary
+}  // namespace qmm
+
+using qmm::fail;
+
+namespace {
+
+struct Span {
+    uintptr_t lo, hi;
+};
+// Bytes from the first to the last element of [batch, tokens, heads, dim] at the given strides (none negative).
+Span span_of(const void *p, const qmm_rotary_args &a, int heads, const int64_t *stride, int64_t esize) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+    const int64_t last = (a.batch - 1) * stride[0] + (a.tokens - 1) * stride[1] + (heads - 1) * stride[2] + a.dim;
+    return Span{b, b + (uintptr_t)(last * esize)};
+}
+bool overlap(const Span &a, const Span &b) { return a.lo < b.hi && b.lo < a.hi; }
+bool same_strides(const int64_t *a, const int64_t *b) { return a[0] == b[0] && a[1] == b[1] && a[2] == b[2]; }
+
+// Whether some two heads of [batch, tokens, heads] share an element: each dimension's stride must reach past the
+// extent of those with smaller strides.
+bool self_overlap(const qmm_rotary_args &a, int heads, const int64_t *stride) {
+    struct D {
+        int64_t n, s;
+    } d[3] = {{a.batch, stride[0]}, {a.tokens, stride[1]}, {heads, stride[2]}};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (d[j].s < d[i].s) {
+                const D t = d[i];
+                d[i] = d[j];
+                d[j] = t;
+            }
+    int64_t extent = a.dim;
+    for (const D &x : d) {
+        if (x.n <= 1) continue;
+        if (x.s < extent) return true;
+        extent += (x.n - 1) * x.s;
+    }
+    return false;
+}
+
+// Whether two operands are certain to share no element: apart in memory, or side by side inside one buffer (a fused
+// projection): the same batch and token strides and, within a token, one after the other or alternating head by head.
+bool apart(const qmm_rotary_args &a, const void *p, int ph, const int64_t *ps, const void *q, int qh, const int64_t *qs, int64_t esize) {
+    if (!overlap(span_of(p, a, ph, ps, esize), span_of(q, a, qh, qs, esize))) return true;
+    if (ps[0] != qs[0] || ps[1] != qs[1] || self_overlap(a, ph, ps) || self_overlap(a, qh, qs)) return false;
+    if (reinterpret_cast<uintptr_t>(p) > reinterpret_cast<uintptr_t>(q)) return apart(a, q, qh, qs, p, ph, ps, esize);
+    const int64_t bytes = (int64_t)(reinterpret_cast<uintptr_t>(q) - reinterpret_cast<uintptr_t>(p));
+    if (bytes % esize) return false;
+    const int64_t d = bytes / esize, pe = (ph - 1) * ps[2] + a.dim, qe = (qh - 1) * qs[2] + a.dim;
+    // the smallest stride that separates two tokens (or batches) of an operand
+    int64_t period = INT64_MAX;
+    if (a.tokens > 1 && ps[1] < period) period = ps[1];
+    if (a.batch > 1 && ps[0] < period) period = ps[0];
+    if (d >= pe && d + qe <= period) return true;
+    const int64_t most = ph > qh ? ph : qh;
+    return ps[2] == qs[2] && d >= a.dim && d + a.dim <= ps[2] && (most - 1) * ps[2] + d + a.dim <= period;
+}
+
+}  // namespace
+
+extern "C" qmm_status qmm_qk_norm_rotary(const qmm_rotary_args *p, void *stream) {
+    if (!p) return fail(QMM_ERR_INVALID_ARGUMENT, "rotary: null arguments");
+    qmm_rotary_args a = *p;
+    if (!a.k) a.k_heads = 0;
+    if (a.batch < 0 || a.tokens < 0 || a.q_heads < 0 || a.k_heads < 0 || a.dim <= 0 || a.pairs < 0 || 2 * (int64_t)a.pairs > a.dim || a.axes <= 0 || a.axes > 256)
+        return fail(QMM_ERR_BAD_SHAPE, "rotary: %lld x %lld tokens, %d and %d heads of %d, %d pairs over %d axes", (long long)a.batch,
+                    (long long)a.tokens, a.q_heads, a.k_heads, a.dim, a.pairs, a.axes);
+    if (a.dim > 256) return fail(QMM_ERR_UNSUPPORTED, "rotary: heads of %d columns (at most 256)", a.dim);
+    if (a.elem < QMM_ELEM_BF16 || a.elem > QMM_ELEM_F16 || a.pos_kind < 0 || a.pos_kind > 2)
+        return fail(QMM_ERR_INVALID_ARGUMENT, "rotary: element type %d, position type %d", a.elem, a.pos_kind);
+    if (a.batch == 0 || a.tokens == 0 || a.q_heads + a.k_heads == 0) return QMM_OK;
+    if ((a.q_heads && (!a.q || !a.q_out)) || (a.k_heads && !a.k_out)) return fail(QMM_ERR_INVALID_ARGUMENT, "rotary: null q, k or output");
+    if (a.pairs && (!a.positions || !a.turns || !a.axis)) return fail(QMM_ERR_INVALID_ARGUMENT, "rotary: null positions, turns or axis");
+    const int64_t esize = a.elem == QMM_ELEM_F32 ? 4 : 2;
+    struct Operand {
+        const void *src, *dst;
+        const int64_t *ss, *ds;
+        int heads;
+    } const ops[2] = {{a.q, a.q_out, a.q_stride, a.q_out_stride, a.q_heads}, {a.k, a.k_out, a.k_stride, a.k_out_stride, a.k_heads}};
+    for (const Operand &o : ops) {
+        if (!o.heads) continue;
+        for (int i = 0; i < 3; ++i)
+            if (o.ss[i] < 0 || o.ds[i] < 0) return fail(QMM_ERR_BAD_SHAPE, "rotary: negative stride");
+        if (reinterpret_cast<uintptr_t>(o.src) % esize || reinterpret_cast<uintptr_t>(o.dst) % esize)
+            return fail(QMM_ERR_MISALIGNED, "rotary: a pointer is not aligned to its element");
+        if (self_overlap(a, o.heads, o.ds)) return fail(QMM_ERR_BAD_SHAPE, "rotary: the output's strides make heads overlap");
+    }
+    // In place (each head is read whole before it is written) or apart.
+    for (const Operand &o : ops) {
+        if (!o.heads) continue;
+        if (!(o.src == o.dst && same_strides(o.ss, o.ds)) && !apart(a, o.src, o.heads, o.ss, o.dst, o.heads, o.ds, esize))
+            return fail(QMM_ERR_INVALID_ARGUMENT, "rotary: an output overlaps its input without being it");
+    }
+    if (a.q_heads && a.k_heads &&
+        (!apart(a, a.q_out, a.q_heads, a.q_out_stride, a.k_out, a.k_heads, a.k_out_stride, esize) ||
+         !apart(a, a.q_out, a.q_heads, a.q_out_stride, a.k, a.k_heads, a.k_stride, esize) ||
+         !apart(a, a.k_out, a.k_heads, a.k_out_stride, a.q, a.q_heads, a.q_stride, esize)))
+        return fail(QMM_ERR_INVALID_ARGUMENT, "rotary: an output overlaps the other operand");
+    const int64_t wsize = esize;
+    if (reinterpret_cast<uintptr_t>(a.q_weight) % wsize || reinterpret_cast<uintptr_t>(a.k_weight) % wsize ||
+        reinterpret_cast<uintptr_t>(a.turns) % 4 || reinterpret_cast<uintptr_t>(a.positions) % (a.pos_kind == 1 ? 8 : 4))
+        return fail(QMM_ERR_MISALIGNED, "rotary: weights, turns or positions are not aligned to their element");
+    const qmm_status s = qmm::check_device();
+    if (s != QMM_OK) return s;
+    bool fast = a.dim % 8 == 0 && (a.adjacent || a.pairs % 4 == 0);
+    const uintptr_t quad = (uintptr_t)(4 * esize);
+    for (const Operand &o : ops) {
+        if (!o.heads) continue;
+        fast = fast && reinterpret_cast<uintptr_t>(o.src) % quad == 0 && reinterpret_cast<uintptr_t>(o.dst) % quad == 0;
+        for (int i = 0; i < 3; ++i) fast = fast && o.ss[i] % 4 == 0 && o.ds[i] % 4 == 0;
+    }
+    fast = fast && reinterpret_cast<uintptr_t>(a.q_weight) % quad == 0 && reinterpret_cast<uintptr_t>(a.k_weight) % quad == 0;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a.elem == QMM_ELEM_F32) return qmm::rotary::launch<float>(a, fast, st);
+    if (a.elem == QMM_ELEM_F16) return qmm::rotary::launch<qmm::F16>(a, fast, st);
+    return qmm::rotary::launch<qmm::Bf16>(a, fast, st);
+}
