@@ -3,49 +3,55 @@
 //   x' = residual_scale * x + gate * h
 //   n  = norm_pre(x') * pre_weight * (1 + scale) + shift
 // HBM-bound: x and branch are read once, x' and n (or its MXFP4 codes) written
-// once.  One CTA per row: the row stays in registers (eight columns a vector, one
-// to four vectors a thread), so mean and variance are two passes over registers,
-// and each statistic costs one shuffle tree, one shared slot a warp and one
-// barrier.  All loads of the row are issued before the first reduction.
-// Rows that are not 16-byte aligned use the same kernel with columns dealt out
-// one by one (thread t holds columns t, t + T, ...), which keeps accesses of a
-// warp consecutive.
+// once; the weights and modulation stay in L1.  A CTA takes a row at a time and
+// keeps it in registers (eight columns a vector, up to four vectors a thread), so
+// mean and variance are two passes over registers, and each statistic costs one
+// shuffle tree, one shared slot a warp and one barrier.  The grid is what is
+// resident at once; each CTA loads its next row while it works on this one.
+// Rows that are not 16-byte aligned take a kernel with columns dealt out one by
+// one (thread t holds columns t, t + T, ...), which keeps accesses of a warp
+// consecutive.
+#include <algorithm>
+
 #include "qmm_internal.h"
 #include "qmm_mx4.cuh"
 
 namespace qmm {
 namespace gnorm {
 
-// Eight elements of a runtime type at an aligned address, kept raw until used.
+// Eight elements of a 16-bit (BYTES 2) or 32-bit type at an aligned address, raw until used.
+template <int BYTES>
 struct Raw8 {
-    uint4 a, b;
+    uint4 w[BYTES / 2];
 };
-__device__ __forceinline__ Raw8 load_raw8(const void *p, int elem, int64_t index) {
-    Raw8 r{};
-    if (elem == QMM_ELEM_F32) {
-        const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const float *>(p) + index);
-        r.a = q[0];
-        r.b = q[1];
-    } else {
-        r.a = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + index);
-    }
+template <int BYTES>
+__device__ __forceinline__ Raw8<BYTES> load_raw8(const void *p, int64_t index) {
+    Raw8<BYTES> r;
+    const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p) + index * BYTES);
+#pragma unroll
+    for (int i = 0; i < BYTES / 2; ++i) r.w[i] = q[i];
     return r;
 }
-__device__ __forceinline__ void raw8_to_f32(const Raw8 &r, int elem, float (&v)[8]) {
-    if (elem == QMM_ELEM_F32) {
+template <int BYTES>
+__device__ __forceinline__ void raw8_to_f32(const Raw8<BYTES> &r, bool f16, float (&v)[8]) {
+    if constexpr (BYTES == 4) {
         Vec8<float> t;
-        t.w[0] = r.a;
-        t.w[1] = r.b;
+        t.w[0] = r.w[0];
+        t.w[1] = r.w[1];
         vec8_to_f32(t, v);
-    } else if (elem == QMM_ELEM_F16) {
+    } else if (f16) {
         Vec8<F16> t;
-        t.w[0] = r.a;
+        t.w[0] = r.w[0];
         vec8_to_f32(t, v);
     } else {
         Vec8<Bf16> t;
-        t.w[0] = r.a;
+        t.w[0] = r.w[0];
         vec8_to_f32(t, v);
     }
+}
+__device__ __forceinline__ void load8(const void *p, int elem, int64_t index, float (&v)[8]) {
+    if (elem == QMM_ELEM_F32) raw8_to_f32(load_raw8<4>(p, index), false, v);
+    else raw8_to_f32(load_raw8<2>(p, index), elem == QMM_ELEM_F16, v);
 }
 __device__ __forceinline__ float load_elem(const void *p, int elem, int64_t i) {
     if (elem == QMM_ELEM_F32) return static_cast<const float *>(p)[i];
@@ -53,200 +59,276 @@ __device__ __forceinline__ float load_elem(const void *p, int elem, int64_t i) {
     return elem_to_f32(static_cast<const Bf16 *>(p)[i]);
 }
 
-template <typename T, int VPT, int MAXT, bool VEC>
-__global__ void __launch_bounds__(MAXT) gated_norm_kernel(const qmm_gated_norm_args a, const int64_t rows_per_group) {
-    __shared__ float red[4][32];
-    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads >> 5;
-    const int64_t row = blockIdx.x, hidden = a.hidden;
-    const int64_t group = row / rows_per_group;
-    const float inv_hidden = 1.0f / (float)hidden;
-
-    auto column = [&](int i, int q) -> int64_t {
-        return VEC ? (int64_t)(i * threads + tid) * 8 + q : (int64_t)(i * 8 + q) * threads + tid;
-    };
-    // v[i][q] = p[base + column], 0 past the row.
-    auto load_row = [&](const void *p, int elem, int64_t base, float (&v)[VPT][8]) {
-        if constexpr (VEC) {
-            Raw8 raw[VPT];
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) {
-                raw[i] = Raw8{};
-                if (column(i, 0) < hidden) raw[i] = load_raw8(p, elem, base + column(i, 0));
-            }
-#pragma unroll
-            for (int i = 0; i < VPT; ++i) raw8_to_f32(raw[i], elem, v[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VPT; ++i)
-#pragma unroll
-                for (int q = 0; q < 8; ++q) v[i][q] = column(i, q) < hidden ? load_elem(p, elem, base + column(i, q)) : 0.0f;
-        }
-    };
-    int phase = 0;
-    auto row_sum = [&](float s) {
+// Sums over a row: a CTA holds it in VPT x 8 columns a thread.  Four slots taken in
+// turn: a slot is written again three barriers after its readers passed theirs.
+struct RowSum {
+    float (&red)[4][32];
+    int slot = 0;
+    __device__ __forceinline__ float operator()(float s) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (warps > 1) {
-            if (lane == 0) red[phase][warp] = s;
+            if (lane == 0) red[slot][warp] = s;
             __syncthreads();
             s = 0.0f;
-            for (int w = 0; w < warps; ++w) s += red[phase][w];  // the same order in every thread
-            ++phase;
+            for (int w = 0; w < warps; ++w) s += red[slot][w];  // the same order in every thread
+            slot = (slot + 1) & 3;
         }
         return s;
-    };
-    // v = norm(v); columns past the row stay 0 for the sums.
-    auto normalise = [&](float (&v)[VPT][8], int kind) {
-        if (kind == QMM_NORM_LAYER) {
-            float s = 0.0f;
-#pragma unroll
-            for (int i = 0; i < VPT; ++i)
-#pragma unroll
-                for (int q = 0; q < 8; ++q) s += v[i][q];
-            const float mean = row_sum(s) * inv_hidden;
-#pragma unroll
-            for (int i = 0; i < VPT; ++i)
-#pragma unroll
-                for (int q = 0; q < 8; ++q) v[i][q] = column(i, q) < hidden ? v[i][q] - mean : 0.0f;
-        }
+    }
+};
+
+// v = norm(v); columns past the row (valid(i, q) false) are 0 and stay 0.
+template <int VPT, typename Valid>
+__device__ __forceinline__ void normalise(float (&v)[VPT][8], int kind, float inv_hidden, float eps, RowSum &row_sum, const Valid &valid) {
+    if (kind == QMM_NORM_LAYER) {
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
-            for (int q = 0; q < 8; ++q) s = fmaf(v[i][q], v[i][q], s);
-        const float r = rsqrtf(row_sum(s) * inv_hidden + a.eps);
+            for (int q = 0; q < 8; ++q) s += v[i][q];
+        const float mean = row_sum(s) * inv_hidden;
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
-            for (int q = 0; q < 8; ++q) v[i][q] *= r;
-    };
+            for (int q = 0; q < 8; ++q) v[i][q] = valid(i, q) ? v[i][q] - mean : 0.0f;
+    }
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s = fmaf(v[i][q], v[i][q], s);
+    const float r = rsqrtf(row_sum(s) * inv_hidden + eps);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[i][q] *= r;
+}
 
-    constexpr int kElem = sizeof(T) == 4 ? (int)QMM_ELEM_F32 : 0;
-    const int x_elem = sizeof(T) == 4 ? kElem : a.x_elem;
-    auto store_row = [&](void *p, int64_t base, const float (&v)[VPT][8]) {
-        T *o = static_cast<T *>(p) + base;
+// Every row of every operand 16-byte aligned, hidden a multiple of 8.
+template <typename T, int BBYTES, int VPT, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group) {
+    __shared__ float red[4][32];
+    RowSum row_sum{red};
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
+    const int hidden = (int)a.hidden;
+    const float inv_hidden = 1.0f / (float)hidden;
+    auto column = [&](int i) { return (i * threads + tid) * 8; };
+    auto valid = [&](int i, int) { return column(i) < hidden; };
+    constexpr int XB = (int)sizeof(T);
+    const bool xf16 = a.x_elem == QMM_ELEM_F16, bf16_branch = a.branch_elem != QMM_ELEM_F16;
+
+    Raw8<XB> rx[VPT];
+    Raw8<BBYTES> rb[VPT];
+    auto fetch = [&](int64_t row) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            if constexpr (VEC) {
-                if (column(i, 0) < hidden) store_vec8(o + column(i, 0), v[i]);
-            } else {
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (column(i, q) < hidden) o[column(i, q)] = elem_from_f32<T>(v[i][q]);
+            rx[i] = Raw8<XB>{};
+            rb[i] = Raw8<BBYTES>{};
+            if (column(i) < hidden) {
+                rx[i] = load_raw8<XB>(a.x, row * a.x_stride + column(i));
+                if (a.branch) rb[i] = load_raw8<BBYTES>(a.branch, row * a.branch_stride + column(i));
             }
         }
     };
-
-    float x[VPT][8];
-    load_row(a.x, x_elem, row * a.x_stride, x);
-    if (a.branch) {
-        float h[VPT][8], w[VPT][8], g[VPT][8];
-        load_row(a.branch, a.branch_elem, row * a.branch_stride, h);
-        if (a.post_weight) load_row(a.post_weight, a.vec_elem, 0, w);
-        if (a.gate) load_row(a.gate, a.vec_elem, group * a.gate_stride, g);
-        if (a.post != QMM_NORM_NONE) normalise(h, a.post);
+    auto store = [&](void *p, int64_t base, const float (&v)[VPT][8]) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
+            if (column(i) < hidden) store_vec8(static_cast<T *>(p) + base + column(i), v[i]);
+    };
+    // v[i][q] = f(v[i][q], vec[base + column])
+    auto with = [&](const void *vec, int64_t base, float (&v)[VPT][8], auto f) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                float t = h[i][q];
-                if (a.post_weight) t *= w[i][q];
-                if (a.gate) t *= g[i][q];
-                x[i][q] = fmaf(a.residual_scale, x[i][q], t);
+        for (int i = 0; i < VPT; ++i) {
+            if (column(i) < hidden) {
+                float w[8];
+                load8(vec, a.vec_elem, base + column(i), w);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[i][q] = f(v[i][q], w[q]);
             }
-    } else {
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-            for (int q = 0; q < 8; ++q) x[i][q] *= a.residual_scale;
-    }
-    if (a.x_out) store_row(a.x_out, row * a.x_out_stride, x);
-    if (!a.n_out && !a.n_codes) return;
-    if (a.pre != QMM_NORM_NONE) normalise(x, a.pre);
-    if (a.pre_weight) {
-        float w[VPT][8];
-        load_row(a.pre_weight, a.vec_elem, 0, w);
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-            for (int q = 0; q < 8; ++q) x[i][q] *= w[i][q];
-    }
-    if (a.scale) {
-        float w[VPT][8];
-        load_row(a.scale, a.vec_elem, group * a.scale_stride, w);
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-            for (int q = 0; q < 8; ++q) x[i][q] *= 1.0f + w[i][q];
-    }
-    if (a.shift) {
-        float w[VPT][8];
-        load_row(a.shift, a.vec_elem, group * a.shift_stride, w);
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-            for (int q = 0; q < 8; ++q) x[i][q] += w[i][q];
-    }
-    if (a.n_out) {
-        store_row(a.n_out, row * a.n_out_stride, x);
-        return;
-    }
-    // MXFP4: columns past the row are zeros of its last block.
+        }
+    };
     const int64_t pitch = mx4_pitch(hidden), tiles = mx4_scale_tiles(hidden);
+
+    fetch(blockIdx.x);
+    for (uint32_t row = blockIdx.x; row < (uint32_t)a.rows; row += gridDim.x) {
+        const uint32_t group = row / rows_per_group;
+        float x[VPT][8], h[VPT][8];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        if constexpr (VEC) {
-            if (column(i, 0) >= hidden) {
+        for (int i = 0; i < VPT; ++i) {
+            raw8_to_f32(rx[i], xf16, x[i]);
+            raw8_to_f32(rb[i], !bf16_branch, h[i]);
+        }
+        if (row + gridDim.x < (uint32_t)a.rows) fetch((int64_t)row + gridDim.x);
+        if (a.branch) {
+            if (a.post != QMM_NORM_NONE) normalise(h, a.post, inv_hidden, a.eps, row_sum, valid);
+            if (a.post_weight) with(a.post_weight, 0, h, [](float v, float w) { return v * w; });
+            if (a.gate) with(a.gate, group * a.gate_stride, h, [](float v, float w) { return v * w; });
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) x[i][q] = fmaf(a.residual_scale, x[i][q], h[i][q]);
+        if (a.x_out) store(a.x_out, row * a.x_out_stride, x);
+        if (!a.n_out && !a.n_codes) continue;
+        if (a.pre != QMM_NORM_NONE) normalise(x, a.pre, inv_hidden, a.eps, row_sum, valid);
+        if (a.pre_weight) with(a.pre_weight, 0, x, [](float v, float w) { return v * w; });
+        if (a.scale) with(a.scale, group * a.scale_stride, x, [](float v, float w) { return fmaf(v, w, v); });
+        if (a.shift) with(a.shift, group * a.shift_stride, x, [](float v, float w) { return v + w; });
+        if (a.n_out) {
+            store(a.n_out, row * a.n_out_stride, x);
+            continue;
+        }
+        // MXFP4: columns past the row are zeros of its last block.
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = column(i);
+            if (c >= hidden) {
 #pragma unroll
                 for (int q = 0; q < 8; ++q) x[i][q] = 0.0f;
             }
             uint32_t codes;
             const uint32_t e = mx4_encode8(x[i], &codes);
-            const int64_t c = column(i, 0);
             if (c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = codes;
             uint32_t word = e << (8 * ((lane >> 2) & 3));
             word |= __shfl_xor_sync(0xffffffffu, word, 4);
             word |= __shfl_xor_sync(0xffffffffu, word, 8);
             const int64_t b = c / kMxBlock;
-            if ((lane & 15) == 0 && b < tiles * 4)
-                *reinterpret_cast<uint32_t *>(a.n_scales + mx4_scale_offset(row, b, tiles)) = word;
-        } else {
+            if ((lane & 15) == 0 && b < tiles * 4) *reinterpret_cast<uint32_t *>(a.n_scales + mx4_scale_offset(row, b, tiles)) = word;
+        }
+    }
+}
+
+// Any alignment and width.
+template <typename T, int VPT, int MAXT>
+__global__ void __launch_bounds__(MAXT) gated_norm_any_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group) {
+    __shared__ float red[4][32];
+    RowSum row_sum{red};
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
+    const int64_t row = blockIdx.x;
+    const int hidden = (int)a.hidden;
+    const int64_t group = (uint32_t)row / rows_per_group;
+    const float inv_hidden = 1.0f / (float)hidden;
+    auto column = [&](int i, int q) { return (i * 8 + q) * threads + tid; };
+    auto valid = [&](int i, int q) { return column(i, q) < hidden; };
+    auto load = [&](const void *p, int elem, int64_t base, float (&v)[VPT][8]) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {  // the warp's 32 lanes hold one block
-                const int64_t c = column(i, q);
-                const float v = c < hidden ? x[i][q] : 0.0f;
-                uint32_t m = __float_as_uint(v) & 0x7FFFFFFFu;
+        for (int i = 0; i < VPT; ++i)
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                const uint32_t e = mx4_scale_code(m);
-                const float one[8] = {v * mx4_inverse_scale(e), 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t word = e == 255u ? 0u : (mx4_pack8(one) & 15u) << (4 * (lane & 7));
-                word |= __shfl_xor_sync(0xffffffffu, word, 1);
-                word |= __shfl_xor_sync(0xffffffffu, word, 2);
-                word |= __shfl_xor_sync(0xffffffffu, word, 4);
-                if ((lane & 7) == 0 && c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = word;
-                const int64_t b = c / kMxBlock;
-                if (lane == 0 && b < tiles * 4) a.n_scales[mx4_scale_offset(row, b, tiles)] = (uint8_t)e;
-            }
+            for (int q = 0; q < 8; ++q) v[i][q] = valid(i, q) ? load_elem(p, elem, base + column(i, q)) : 0.0f;
+    };
+    auto store = [&](void *p, int64_t base, const float (&v)[VPT][8]) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (valid(i, q)) static_cast<T *>(p)[base + column(i, q)] = elem_from_f32<T>(v[i][q]);
+    };
+    auto with = [&](const void *vec, int64_t base, float (&v)[VPT][8], auto f) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (valid(i, q)) v[i][q] = f(v[i][q], load_elem(vec, a.vec_elem, base + column(i, q)));
+    };
+    float x[VPT][8], h[VPT][8];
+    load(a.x, a.x_elem, row * a.x_stride, x);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) h[i][q] = 0.0f;
+    if (a.branch) {
+        load(a.branch, a.branch_elem, row * a.branch_stride, h);
+        if (a.post != QMM_NORM_NONE) normalise(h, a.post, inv_hidden, a.eps, row_sum, valid);
+        if (a.post_weight) with(a.post_weight, 0, h, [](float v, float w) { return v * w; });
+        if (a.gate) with(a.gate, group * a.gate_stride, h, [](float v, float w) { return v * w; });
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[i][q] = fmaf(a.residual_scale, x[i][q], h[i][q]);
+    if (a.x_out) store(a.x_out, row * a.x_out_stride, x);
+    if (!a.n_out && !a.n_codes) return;
+    if (a.pre != QMM_NORM_NONE) normalise(x, a.pre, inv_hidden, a.eps, row_sum, valid);
+    if (a.pre_weight) with(a.pre_weight, 0, x, [](float v, float w) { return v * w; });
+    if (a.scale) with(a.scale, group * a.scale_stride, x, [](float v, float w) { return fmaf(v, w, v); });
+    if (a.shift) with(a.shift, group * a.shift_stride, x, [](float v, float w) { return v + w; });
+    if (a.n_out) {
+        store(a.n_out, row * a.n_out_stride, x);
+        return;
+    }
+    // MXFP4: a warp's 32 lanes hold one block; columns past the row are zeros of its last block.
+    const int64_t pitch = mx4_pitch(hidden), tiles = mx4_scale_tiles(hidden);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const int c = column(i, q);
+            const float v = c < hidden ? x[i][q] : 0.0f;
+            uint32_t m = __float_as_uint(v) & 0x7FFFFFFFu;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const uint32_t e = mx4_scale_code(m);
+            const float one[8] = {v * mx4_inverse_scale(e), 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            uint32_t word = e == 255u ? 0u : (mx4_pack8(one) & 15u) << (4 * (lane & 7));
+            word |= __shfl_xor_sync(0xffffffffu, word, 1);
+            word |= __shfl_xor_sync(0xffffffffu, word, 2);
+            word |= __shfl_xor_sync(0xffffffffu, word, 4);
+            if ((lane & 7) == 0 && c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = word;
+            const int64_t b = c / kMxBlock;
+            if (lane == 0 && b < tiles * 4) a.n_scales[mx4_scale_offset(row, b, tiles)] = (uint8_t)e;
         }
     }
 }
 
 // Threads a row: whole warps, the fewest that hold it in VPT vectors each.
-template <typename T, int VPT, int MAXT, bool VEC>
-static void launch_as(const qmm_gated_norm_args &a, int64_t rpg, cudaStream_t st) {
-    const int64_t vectors = (a.hidden + 7) / 8;
-    const unsigned threads = (unsigned)(((vectors + VPT - 1) / VPT + 31) / 32 * 32);
-    gated_norm_kernel<T, VPT, MAXT, VEC><<<(unsigned)a.rows, threads, 0, st>>>(a, rpg);
+template <int VPT>
+static unsigned threads_for(int64_t hidden) {
+    const int64_t vectors = (hidden + 7) / 8;
+    return (unsigned)(((vectors + VPT - 1) / VPT + 31) / 32 * 32);
 }
 
-template <typename T, bool VEC>
-static void launch_vec(const qmm_gated_norm_args &a, int64_t rpg, cudaStream_t st) {
-    if (a.hidden <= 1024) launch_as<T, 1, 128, VEC>(a, rpg, st);
-    else if (a.hidden <= 4096) launch_as<T, 2, 256, VEC>(a, rpg, st);
-    else if (a.hidden <= 8192) launch_as<T, 4, 256, VEC>(a, rpg, st);
-    else if (a.hidden <= 16384) launch_as<T, 4, 512, VEC>(a, rpg, st);
-    else launch_as<T, 4, 1024, VEC>(a, rpg, st);
+template <typename T, int BBYTES, int VPT, int MAXT, int MINB>
+static void launch_rows(const qmm_gated_norm_args &a, uint32_t rpg, cudaStream_t st) {
+    auto kernel = gated_norm_kernel<T, BBYTES, VPT, MAXT, MINB>;
+    const unsigned threads = threads_for<VPT>(a.hidden);
+    static int resident[64][33] = {};  // CTAs an SM by device and warps
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
+    int &n = resident[dev][threads / 32];
+    if (n == 0) {
+        int m = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&m, kernel, (int)threads, 0) != cudaSuccess || m < 1) m = 1;
+        n = m;
+    }
+    const unsigned grid = (unsigned)std::min<int64_t>(a.rows, (int64_t)sm_count() * n);
+    kernel<<<grid, threads, 0, st>>>(a, rpg);
+}
+
+template <typename T, int BBYTES>
+static void launch_fast(const qmm_gated_norm_args &a, uint32_t rpg, cudaStream_t st) {
+    if (a.hidden <= 1024) launch_rows<T, BBYTES, 1, 128, 8>(a, rpg, st);
+    else if (a.hidden <= 4096) launch_rows<T, BBYTES, 2, 256, 3>(a, rpg, st);
+    else if (a.hidden <= 8192) launch_rows<T, BBYTES, 4, 256, 1>(a, rpg, st);
+    else if (a.hidden <= 16384) launch_rows<T, BBYTES, 4, 512, 1>(a, rpg, st);
+    else launch_rows<T, BBYTES, 4, 1024, 1>(a, rpg, st);
+}
+
+template <typename T>
+static void launch_any(const qmm_gated_norm_args &a, uint32_t rpg, cudaStream_t st) {
+    const unsigned grid = (unsigned)a.rows;
+    if (a.hidden <= 1024) gated_norm_any_kernel<T, 1, 128><<<grid, threads_for<1>(a.hidden), 0, st>>>(a, rpg);
+    else if (a.hidden <= 4096) gated_norm_any_kernel<T, 2, 256><<<grid, threads_for<2>(a.hidden), 0, st>>>(a, rpg);
+    else if (a.hidden <= 16384) gated_norm_any_kernel<T, 4, 512><<<grid, threads_for<4>(a.hidden), 0, st>>>(a, rpg);
+    else gated_norm_any_kernel<T, 4, 1024><<<grid, threads_for<4>(a.hidden), 0, st>>>(a, rpg);
+}
+
+template <typename T>
+static void launch(const qmm_gated_norm_args &a, bool fast, uint32_t rpg, cudaStream_t st) {
+    if (!fast) launch_any<T>(a, rpg, st);
+    else if (a.branch_elem == QMM_ELEM_F32) launch_fast<T, 4>(a, rpg, st);
+    else launch_fast<T, 2>(a, rpg, st);
 }
 
 }  // namespace gnorm
@@ -345,14 +427,10 @@ extern "C" qmm_status qmm_gated_residual_norm(const qmm_gated_norm_args *p, void
                      aligned_vec(a.pre_weight, 0) && aligned_vec(a.gate, a.gate_stride) && aligned_vec(a.shift, a.shift_stride) &&
                      aligned_vec(a.scale, a.scale_stride);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int64_t rpg = a.rows / a.groups;
-#define QMM_GNORM(T)                                    \
-    (vec ? qmm::gnorm::launch_vec<T, true>(a, rpg, st)  \
-         : qmm::gnorm::launch_vec<T, false>(a, rpg, st))
-    if (a.x_elem == QMM_ELEM_F32) QMM_GNORM(float);
-    else if (a.x_elem == QMM_ELEM_F16) QMM_GNORM(qmm::F16);
-    else QMM_GNORM(qmm::Bf16);
-#undef QMM_GNORM
+    const uint32_t rpg = (uint32_t)(a.rows / a.groups);
+    if (a.x_elem == QMM_ELEM_F32) qmm::gnorm::launch<float>(a, vec, rpg, st);
+    else if (a.x_elem == QMM_ELEM_F16) qmm::gnorm::launch<qmm::F16>(a, vec, rpg, st);
+    else qmm::gnorm::launch<qmm::Bf16>(a, vec, rpg, st);
     qmm::count_launch();
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? QMM_OK : qmm::cuda_fail(e, "gated norm launch");

@@ -4,8 +4,9 @@
 // HBM-bound: q and k are read and written once; positions are a few bytes a
 // token.  A warp takes a token and a run of its heads.  Each lane holds the same
 // four pairs of every head (as two runs of four columns), so the token's sines
-// and cosines are computed once per lane and stay in registers over the heads; a
-// head of 8 U columns takes U lanes, 32 / U heads go at a time.
+// and cosines are computed once per lane and, multiplied with the norm's weight,
+// stay in registers over the heads; a head of 8 U columns takes U lanes, and
+// 32 / U heads (rounded down) go at a time.
 //
 // The angle is positions * turns in turns.  With turns = f + g (leading and
 // trailing term), p = fl(pos f) and e = pos f - p exact by one fma, the fraction
@@ -35,133 +36,170 @@ __device__ __forceinline__ void pair_turn(const qmm_rotary_args &a, int64_t batc
     sincospif(2.0f * t, s, c);
 }
 
-// Four elements at an address aligned to four elements.
+// Eight elements as two runs of four, each at an address aligned to four
+// elements; ADJ: the runs are neighbours at an address aligned to eight.
 template <typename T>
-struct Vec4 {
-    uint32_t w[sizeof(T)];
+struct Runs {
+    uint32_t w[sizeof(T) * 2];
 };
-template <typename T>
-__device__ __forceinline__ Vec4<T> load_vec4(const T *p) {
-    Vec4<T> r;
+template <typename T, bool ADJ>
+__device__ __forceinline__ Runs<T> load_runs(const T *p, int ca, int cb) {
+    Runs<T> r;
     if constexpr (sizeof(T) == 4) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
-        r.w[0] = v.x, r.w[1] = v.y, r.w[2] = v.z, r.w[3] = v.w;
+        const uint4 a = *reinterpret_cast<const uint4 *>(p + ca), b = *reinterpret_cast<const uint4 *>(p + cb);
+        r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
+        r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
+    } else if constexpr (ADJ) {
+        const uint4 a = *reinterpret_cast<const uint4 *>(p + ca);
+        r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
     } else {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        r.w[0] = v.x, r.w[1] = v.y;
+        const uint2 a = *reinterpret_cast<const uint2 *>(p + ca), b = *reinterpret_cast<const uint2 *>(p + cb);
+        r.w[0] = a.x, r.w[1] = a.y, r.w[2] = b.x, r.w[3] = b.y;
     }
     return r;
 }
 template <typename T>
-__device__ __forceinline__ void vec4_to_f32(const Vec4<T> &r, float (&v)[4]) {
+__device__ __forceinline__ void runs_to_f32(const Runs<T> &r, float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r.w[i]);
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.w[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const float2 f = unpack2<T>(r.w[i]);
             v[2 * i] = f.x;
             v[2 * i + 1] = f.y;
         }
     }
 }
-template <typename T>
-__device__ __forceinline__ void store_vec4(T *p, const float (&v)[4]) {
+template <typename T, bool ADJ>
+__device__ __forceinline__ void store_runs(T *p, int ca, int cb, const float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4 *>(p + ca) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4 *>(p + cb) = make_float4(v[4], v[5], v[6], v[7]);
+    } else if constexpr (ADJ) {
+        *reinterpret_cast<uint4 *>(p + ca) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
     } else {
-        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+        *reinterpret_cast<uint2 *>(p + ca) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+        *reinterpret_cast<uint2 *>(p + cb) = make_uint2(pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
     }
 }
 
-// G: lanes a head (a power of two, at least dim / 8).  Needs dim % 8 == 0, with
-// halves pairs % 4 == 0, and every head at an address aligned to four elements.
-template <typename T, int G>
+// The heads [h0, h1) of one operand for one token.
+template <typename T>
+struct Heads {
+    const T *src;
+    T *dst;
+    int64_t src_stride, dst_stride;
+    int h0, h1;
+};
+
+// A warp takes a token and a run of its q and k heads; a head's dim / 8 units go
+// to as many lanes, 32 / units heads at a time.  Needs dim % 8 == 0, with halves
+// pairs % 4 == 0, heads aligned to four elements (ADJ: adjacent pairs, heads
+// aligned to eight).  POW2: dim / 8 is a power of two.
+template <typename T, bool ADJ, bool POW2>
 __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const qmm_rotary_args a, const int heads_per_warp) {
-    constexpr int H = 32 / G;  // heads at a time
-    const int lane = threadIdx.x & 31, u = lane % G, sub = lane / G;
-    const int splits = (a.q_heads + a.k_heads + heads_per_warp - 1) / heads_per_warp;
-    const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const int64_t row = unit / splits;
-    if (row >= a.batch * a.tokens) return;
-    const int64_t batch = row / a.tokens, token = row % a.tokens;
-    const int heads = a.q_heads + a.k_heads;
-    const int h0 = (int)(unit % splits) * heads_per_warp, h1 = min(h0 + heads_per_warp, heads);
-    const bool live = u * 8 < a.dim;
-    // This lane's columns: [ca, ca + 4) and [cb, cb + 4), and their pairs.
-    int ca = u * 8, cb = u * 8 + 4, pair = u * 4;
-    if (!a.adjacent && u * 4 < a.pairs) ca = u * 4, cb = a.pairs + u * 4;
+    const int units = a.dim >> 3, at_a_time = 32 / units;
+    const int lane = threadIdx.x & 31, sub = lane / units, u = lane - sub * units;
+    const uint32_t row = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (row >= (uint32_t)(a.batch * a.tokens)) return;
+    const uint32_t tokens = (uint32_t)a.tokens, batch = row / tokens, token = row - batch * tokens;
+    const int first = blockIdx.y * heads_per_warp, last = first + heads_per_warp;
+    const bool live = sub < at_a_time;
+    int ca = u * 8, cb = u * 8 + 4;
+    const int pair = u * 4;
+    if (!ADJ && pair < a.pairs && !a.adjacent) ca = pair, cb = a.pairs + pair;
     float cs[4], sn[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        cs[i] = 1.0f, sn[i] = 0.0f;
-        if (pair + i < a.pairs) pair_turn(a, batch, token, pair + i, &cs[i], &sn[i]);
-    }
+    bool turned = false;
     const float inv_dim = 1.0f / (float)a.dim;
-    for (int hb = h0; hb < h1; hb += H * kAhead) {
-        Vec4<T> ra[kAhead], rb[kAhead];
+
+    auto run = [&](const Heads<T> &h, const T *weight) {
+        if (h.h0 >= h.h1) return;
+        const T *src = h.src + (int64_t)(h.h0 + sub) * h.src_stride;
+        T *dst = h.dst + (int64_t)(h.h0 + sub) * h.dst_stride;
+        const int64_t src_step = at_a_time * h.src_stride, dst_step = at_a_time * h.dst_stride;
+        // out[even] = r (v[even] A - v[odd] B), out[odd] = r (v[even] C + v[odd] D): weight and turn in one factor
+        float fa[4], fb[4], fc[4], fd[4];
+        for (int hb = h.h0; hb < h.h1; hb += at_a_time * kAhead) {
+            Runs<T> raw[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            const int h = hb + j * H + sub;
-            ra[j] = Vec4<T>{}, rb[j] = Vec4<T>{};
-            if (h < h1 && live) {
-                const bool isq = h < a.q_heads;
-                const T *src = isq ? static_cast<const T *>(a.q) + batch * a.q_stride[0] + token * a.q_stride[1] + h * a.q_stride[2]
-                                   : static_cast<const T *>(a.k) + batch * a.k_stride[0] + token * a.k_stride[1] +
-                                         (h - a.q_heads) * a.k_stride[2];
-                ra[j] = load_vec4(src + ca);
-                rb[j] = load_vec4(src + cb);
+            for (int j = 0; j < kAhead; ++j) {
+                raw[j] = Runs<T>{};
+                if (live && hb + j * at_a_time + sub < h.h1) raw[j] = load_runs<T, ADJ>(src + j * src_step, ca, cb);
             }
-        }
+            if (!turned) {  // (after the first loads are on their way)
+                turned = true;
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            const int h = hb + j * H + sub;
-            const bool isq = h < a.q_heads;
-            float va[4], vb[4];
-            vec4_to_f32(ra[j], va);
-            vec4_to_f32(rb[j], vb);
-            const T *w = static_cast<const T *>(isq ? a.q_weight : a.k_weight);
-            if (a.q_weight || a.k_weight) {  // (the shuffles below take the whole warp)
-                float s = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s = fmaf(va[i], va[i], fmaf(vb[i], vb[i], s));
-#pragma unroll
-                for (int o = G / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                if (w && live) {
-                    const float r = rsqrtf(s * inv_dim + a.eps);
-                    float wa[4], wb[4];
-                    vec4_to_f32(load_vec4(w + ca), wa);
-                    vec4_to_f32(load_vec4(w + cb), wb);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) va[i] *= r * wa[i], vb[i] *= r * wb[i];
+                for (int i = 0; i < 4; ++i) {
+                    cs[i] = 1.0f, sn[i] = 0.0f;
+                    if (live && pair + i < a.pairs) pair_turn(a, batch, token, pair + i, &cs[i], &sn[i]);
                 }
             }
-            if (h < h1 && live) {
-                float oa[4], ob[4];
-                if (a.adjacent) {
+            if (hb == h.h0) {
+                float w[8];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        oa[2 * i] = va[2 * i] * cs[i] - va[2 * i + 1] * sn[i];
-                        oa[2 * i + 1] = va[2 * i] * sn[i] + va[2 * i + 1] * cs[i];
-                        ob[2 * i] = vb[2 * i] * cs[i + 2] - vb[2 * i + 1] * sn[i + 2];
-                        ob[2 * i + 1] = vb[2 * i] * sn[i + 2] + vb[2 * i + 1] * cs[i + 2];
+                for (int i = 0; i < 8; ++i) w[i] = 1.0f;
+                if (weight && live) runs_to_f32(load_runs<T, ADJ>(weight, ca, cb), w);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float we = w[(ADJ || a.adjacent) ? 2 * i : i], wo = w[(ADJ || a.adjacent) ? 2 * i + 1 : i + 4];
+                    fa[i] = we * cs[i], fb[i] = wo * sn[i], fc[i] = we * sn[i], fd[i] = wo * cs[i];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                float v[8];
+                runs_to_f32(raw[j], v);
+                float r = 1.0f;
+                if (weight) {
+                    float s = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s = fmaf(v[i], v[i], s);
+                    if constexpr (POW2) {
+#pragma unroll
+                        for (int o = 16; o > 0; o >>= 1)
+                            if (o < units) s += __shfl_xor_sync(0xffffffffu, s, o);
+                    } else {
+#pragma unroll
+                        for (int o = 1; o < 32; o <<= 1) {
+                            if (o < units) {
+                                const float t = __shfl_down_sync(0xffffffffu, s, o);
+                                if (u + o < units) s += t;
+                            }
+                        }
+                        s = __shfl_sync(0xffffffffu, s, lane - u);
+                    }
+                    r = rsqrtf(s * inv_dim + a.eps);
+                }
+                float o[8];
+                if (ADJ || a.adjacent) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[2 * i] = r * (v[2 * i] * fa[i] - v[2 * i + 1] * fb[i]);
+                        o[2 * i + 1] = r * (v[2 * i] * fc[i] + v[2 * i + 1] * fd[i]);
                     }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        oa[i] = va[i] * cs[i] - vb[i] * sn[i];
-                        ob[i] = va[i] * sn[i] + vb[i] * cs[i];
+                        o[i] = r * (v[i] * fa[i] - v[i + 4] * fb[i]);
+                        o[i + 4] = r * (v[i] * fc[i] + v[i + 4] * fd[i]);
                     }
                 }
-                T *dst = isq ? static_cast<T *>(a.q_out) + batch * a.q_out_stride[0] + token * a.q_out_stride[1] + h * a.q_out_stride[2]
-                             : static_cast<T *>(a.k_out) + batch * a.k_out_stride[0] + token * a.k_out_stride[1] +
-                                   (h - a.q_heads) * a.k_out_stride[2];
-                store_vec4(dst + ca, oa);
-                store_vec4(dst + cb, ob);
+                if (live && hb + j * at_a_time + sub < h.h1) store_runs<T, ADJ>(dst + j * dst_step, ca, cb, o);
             }
+            src += src_step * kAhead;
+            dst += dst_step * kAhead;
         }
-    }
+    };
+    run(Heads<T>{static_cast<const T *>(a.q) + batch * a.q_stride[0] + token * a.q_stride[1],
+                 static_cast<T *>(a.q_out) + batch * a.q_out_stride[0] + token * a.q_out_stride[1], a.q_stride[2], a.q_out_stride[2],
+                 first, min(last, a.q_heads)},
+        static_cast<const T *>(a.q_weight));
+    run(Heads<T>{static_cast<const T *>(a.k) + batch * a.k_stride[0] + token * a.k_stride[1],
+                 static_cast<T *>(a.k_out) + batch * a.k_out_stride[0] + token * a.k_out_stride[1], a.k_stride[2], a.k_out_stride[2],
+                 max(first - a.q_heads, 0), min(last - a.q_heads, a.k_heads)},
+        static_cast<const T *>(a.k_weight));
 }
 
 // Any dim up to 256, any pairs, any alignment: lane l takes pairs l, l + 32, ...
@@ -169,13 +207,11 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const qmm_rotary_ar
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32) rotary_any_kernel(const qmm_rotary_args a, const int heads_per_warp) {
     const int lane = threadIdx.x & 31;
-    const int splits = (a.q_heads + a.k_heads + heads_per_warp - 1) / heads_per_warp;
-    const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const int64_t row = unit / splits;
-    if (row >= a.batch * a.tokens) return;
-    const int64_t batch = row / a.tokens, token = row % a.tokens;
+    const uint32_t row = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (row >= (uint32_t)(a.batch * a.tokens)) return;
+    const uint32_t tokens = (uint32_t)a.tokens, batch = row / tokens, token = row - batch * tokens;
     const int heads = a.q_heads + a.k_heads;
-    const int h0 = (int)(unit % splits) * heads_per_warp, h1 = min(h0 + heads_per_warp, heads);
+    const int h0 = blockIdx.y * heads_per_warp, h1 = min(h0 + heads_per_warp, heads);
     float cs[4], sn[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -235,30 +271,28 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_any_kernel(const qmm_rotar
 }
 
 template <typename T>
-static qmm_status launch(const qmm_rotary_args &a, bool fast, cudaStream_t st) {
-    const int heads = a.q_heads + a.k_heads;
-    int g = 4;
-    while (g * 8 < a.dim) g *= 2;
-    const int at_a_time = fast ? 32 / g : 1;
+static qmm_status launch(const qmm_rotary_args &a, bool fast, bool wide, cudaStream_t st) {
+    const int heads = a.q_heads + a.k_heads, units = a.dim / 8;
+    const int at_a_time = fast ? 32 / units : 1;
     // Heads a warp: all of a token's where the tokens alone fill the machine, so
     // that its sines are computed once; fewer where they do not, down to the
     // heads that a warp handles at a time.
     const int64_t rows = a.batch * a.tokens;
-    int64_t splits = 1;
+    if (rows > INT32_MAX) return fail(QMM_ERR_UNSUPPORTED, "rotary: %lld tokens are past the launch limits", (long long)rows);
     const int64_t most = (heads + at_a_time - 1) / at_a_time;
+    int64_t splits = 1;
     while (splits < most && rows * splits < (int64_t)sm_count() * 16) splits *= 2;
     if (splits > most) splits = most;
     int per = (int)((heads + splits - 1) / splits);
     per = (per + at_a_time - 1) / at_a_time * at_a_time;
-    splits = (heads + per - 1) / per;
-    const int64_t blocks = (rows * splits + kWarps - 1) / kWarps;
-    if (blocks > INT32_MAX) return fail(QMM_ERR_UNSUPPORTED, "rotary: %lld tokens are past the launch limits", (long long)rows);
-    const unsigned grid = (unsigned)blocks;
+    const dim3 grid((unsigned)((rows + kWarps - 1) / kWarps), (unsigned)((heads + per - 1) / per), 1);
+    const bool pow2 = fast && (units & (units - 1)) == 0;
+    if (grid.y > 65535) return fail(QMM_ERR_UNSUPPORTED, "rotary: %d heads are past the launch limits", heads);
     if (!fast) rotary_any_kernel<T><<<grid, kWarps * 32, 0, st>>>(a, per);
-    else if (g == 4) rotary_kernel<T, 4><<<grid, kWarps * 32, 0, st>>>(a, per);
-    else if (g == 8) rotary_kernel<T, 8><<<grid, kWarps * 32, 0, st>>>(a, per);
-    else if (g == 16) rotary_kernel<T, 16><<<grid, kWarps * 32, 0, st>>>(a, per);
-    else rotary_kernel<T, 32><<<grid, kWarps * 32, 0, st>>>(a, per);
+    else if (wide && pow2) rotary_kernel<T, true, true><<<grid, kWarps * 32, 0, st>>>(a, per);
+    else if (wide) rotary_kernel<T, true, false><<<grid, kWarps * 32, 0, st>>>(a, per);
+    else if (pow2) rotary_kernel<T, false, true><<<grid, kWarps * 32, 0, st>>>(a, per);
+    else rotary_kernel<T, false, false><<<grid, kWarps * 32, 0, st>>>(a, per);
     count_launch();
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? QMM_OK : cuda_fail(e, "rotary launch");
@@ -369,16 +403,26 @@ extern "C" qmm_status qmm_qk_norm_rotary(const qmm_rotary_args *p, void *stream)
         return fail(QMM_ERR_MISALIGNED, "rotary: weights, turns or positions are not aligned to their element");
     const qmm_status s = qmm::check_device();
     if (s != QMM_OK) return s;
-    bool fast = a.dim % 8 == 0 && (a.adjacent || a.pairs % 4 == 0);
+    // fast: runs of four elements; wide: adjacent pairs, runs of eight (16 bytes of a 16-bit type)
+    bool fast = a.dim % 8 == 0 && (a.adjacent || a.pairs % 4 == 0), wide = a.adjacent != 0;
     const uintptr_t quad = (uintptr_t)(4 * esize);
+    auto judge = [&](const void *p, const int64_t *strides) {
+        fast = fast && reinterpret_cast<uintptr_t>(p) % quad == 0;
+        wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+        for (int i = 0; strides && i < 3; ++i) {
+            fast = fast && strides[i] % 4 == 0;
+            wide = wide && (strides[i] * esize) % 16 == 0;
+        }
+    };
     for (const Operand &o : ops) {
         if (!o.heads) continue;
-        fast = fast && reinterpret_cast<uintptr_t>(o.src) % quad == 0 && reinterpret_cast<uintptr_t>(o.dst) % quad == 0;
-        for (int i = 0; i < 3; ++i) fast = fast && o.ss[i] % 4 == 0 && o.ds[i] % 4 == 0;
+        judge(o.src, o.ss);
+        judge(o.dst, o.ds);
     }
-    fast = fast && reinterpret_cast<uintptr_t>(a.q_weight) % quad == 0 && reinterpret_cast<uintptr_t>(a.k_weight) % quad == 0;
+    judge(a.q_weight, nullptr);
+    judge(a.k_weight, nullptr);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a.elem == QMM_ELEM_F32) return qmm::rotary::launch<float>(a, fast, st);
-    if (a.elem == QMM_ELEM_F16) return qmm::rotary::launch<qmm::F16>(a, fast, st);
-    return qmm::rotary::launch<qmm::Bf16>(a, fast, st);
+    if (a.elem == QMM_ELEM_F32) return qmm::rotary::launch<float>(a, fast, wide, st);
+    if (a.elem == QMM_ELEM_F16) return qmm::rotary::launch<qmm::F16>(a, fast, wide, st);
+    return qmm::rotary::launch<qmm::Bf16>(a, fast, wide, st);
 }
