@@ -14,13 +14,14 @@
 // two of them).  A feature tile of 192 starts in the middle of a 128-row scale tile
 // every other time; the MMA's scale address then starts two columns in.
 //
-// Warp roles (one persistent CTA per SM): 8 epilogue warps (two per lane quadrant,
-// each half of the columns), a producer warp (TMA for codes, bulk copies for
-// scales), an MMA warp (one elected lane issues copies, MMAs and commits).  Two
+// Warp roles (one persistent CTA per SM): 16 epilogue warps (four per lane quadrant,
+// dealing its columns out in chunks of 32), a producer warp (TMA for codes, bulk
+// copies for scales), an MMA warp (one elected lane issues copies, MMAs and commits).  Two
 // accumulators, so a tile's epilogue overlaps the next tile's main loop.  Scale
 // slots in tensor memory are tied to the shared-memory stages: a stage refilled
 // means that the MMAs that read its slot are complete.  Every wait is bounded.
 #include <algorithm>
+#include <climits>
 #include <mutex>
 
 #include "qmm_epilogue.cuh"
@@ -34,10 +35,12 @@ constexpr int kTM = 128;         // tokens a tile
 constexpr int kBK = 256;         // columns a stage
 constexpr int kRowBytes = 128;   // codes of a row in a stage
 constexpr int kSfTile = 512;     // scales of 128 rows x 4 blocks
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;
 constexpr int kProducer = kEpiWarps, kMma = kEpiWarps + 1;
 constexpr int kThreads = (kEpiWarps + 2) * 32;
+constexpr int kMaxChunks = 2;    // of an epilogue warp in a tile
 constexpr int kChunk = 32;       // columns an epilogue step
+constexpr int kGroups = kEpiWarps / 4;  // epilogue warps on each lane quadrant: chunk c is group c % kGroups
 
 template <int TN>
 struct Cfg {
@@ -48,8 +51,8 @@ struct Cfg {
     static constexpr int kSfaBytes = 2 * kSfTile;
     static constexpr int kSfbBytes = 2 * kBTiles * kSfTile;
     static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
-    static constexpr int kOutBytes = kEpiWarps * 2 * kChunk * 64;  // two 32 x 32 bf16 buffers a warp
-    static constexpr int kVecBytes = kEpiWarps * 2 * kChunk * 4;   // bias and gate of a chunk, a warp
+    static constexpr int kOutBytes = kEpiWarps * kChunk * 64;  // a 32 x 32 bf16 buffer a warp
+    static constexpr int kVecBytes = kEpiWarps * kMaxChunks * 2 * kChunk * 4;  // bias and gate of a warp's chunks
     static constexpr int kSfCols = 2 * 4 * (1 + kBTiles);          // tensor-memory columns of a stage's scales
     static constexpr int kFit = (232448 - 1024 - 512 - kOutBytes - kVecBytes) / kStageBytes;
     static constexpr int kSlots = (512 - 2 * TN) / kSfCols;
@@ -61,7 +64,7 @@ struct Cfg {
     static constexpr int kSfbOff = kSfaOff + kStages * kSfaBytes;
     static constexpr int kVecOff = kSfbOff + kStages * kSfbBytes;
     static constexpr int kBarOff = kVecOff + kVecBytes;
-    static constexpr int kNumBars = 2 * kStages + 4 + 1 + kEpiWarps * 2;
+    static constexpr int kNumBars = 2 * kStages + 4 + 1 + kEpiWarps;
     static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
     static constexpr int kSfCol0 = 2 * TN;
     static_assert(kStages >= 2 && kSmemBytes <= 232448, "shared memory");
@@ -77,9 +80,15 @@ struct Params {
     int32_t nkb, sf_tiles;       // stages along k; scale tiles along k
     int32_t m_tiles, n_tiles;
     int32_t b_row_tiles;         // 128-row scale tiles of W
-    int32_t tma_out;             // y (and the residual) by TMA: n % 8 == 0
+    int32_t tma_out;             // y (and the residual) by TMA: rows on 16-byte boundaries
     uint32_t *err;
 };
+
+// Tile t of the persistent loop.  (Patches of 4, 8 and 16 tiles of tokens measured the same.)
+__device__ __forceinline__ void tile_at(const Params &p, int t, int &mt, int &nt) {
+    nt = t / p.m_tiles;
+    mt = t - nt * p.m_tiles;
+}
 
 // Shared-memory descriptor of a 512-byte scale tile (32 rows of 16 bytes, no
 // swizzle: 8-row groups 128 bytes apart).
@@ -102,6 +111,183 @@ __device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t a, uint64_t b, 
         : "memory");
 }
 
+// t * sigmoid(z) of two values: both activations in one exponential and one
+// reciprocal a value (GELU's 0.5 (1 + tanh u) is sigmoid(2 u)).  The fast forms are
+// good to a few 2^-22 of the result, far below its rounding to bf16; past their range
+// they give 0 or t.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool GELU>
+__device__ __forceinline__ float2 activate(float2 t) {
+    const float2 zero = make_float2(0.0f, 0.0f);
+    constexpr float kLog2e = 1.4426950408889634f, kGelu = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+    float2 z;  // -z log2(e)
+    if constexpr (GELU) {
+        const float2 a = make_float2(-kGelu * kLog2e, -kGelu * kLog2e), b = make_float2(-kGelu * kLog2e * 0.044715f, -kGelu * kLog2e * 0.044715f);
+        z = fma_f32x2(fma_f32x2(fma_f32x2(t, t, zero), b, a), t, zero);
+    } else {
+        z = fma_f32x2(t, make_float2(-kLog2e, -kLog2e), zero);
+    }
+    const float2 d = add_f32x2(make_float2(exp2_fast(z.x), exp2_fast(z.y)), make_float2(1.0f, 1.0f));
+    return make_float2(t.x * rcp_fast(d.x), t.y * rcp_fast(d.y));
+}
+
+// What an epilogue warp owns in shared memory.
+struct ChunkOut {
+    uint8_t *stage;     // 32 tokens x 32 features of bf16: 64 bytes a token, 16-byte cells swizzled
+    float *vec;         // bias[32], gate[32] of each of the tile's chunks
+    uint64_t *res_full; // a residual chunk landed in `stage`
+};
+
+__device__ __forceinline__ void request_residual(const CUtensorMap *tmap_res, const ChunkOut &o, int f0, int m0) {
+    if ((threadIdx.x & 31) == 0) {
+        bulk_wait_read<0>();  // the last store has left the buffer
+        mbar_arrive_expect_tx(o.res_full, kChunk * 64);
+        tma_load_2d(o.stage, tmap_res, o.res_full, f0, m0);
+    }
+}
+
+// One warp's 32 tokens x 32 features, from the accumulators in r (a token a lane)
+// through its staging buffer to y.
+__device__ __forceinline__ void chunk_finish(const Params &p, const CUtensorMap *tmap_y, const ChunkOut &o, const float *vec, uint32_t (&r)[32],
+                                             int f0, int m0, bool res_tma) {
+    const int lane = threadIdx.x & 31, row = m0 + lane;
+    const float4 *const bias = reinterpret_cast<const float4 *>(vec), *const gate = bias + kChunk / 4;
+    // Each step over all 32 features: its branch is taken once, and the exponentials overlap.
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float4 b4 = bias[i];
+        v[4 * i] = __uint_as_float(r[4 * i]) + b4.x;
+        v[4 * i + 1] = __uint_as_float(r[4 * i + 1]) + b4.y;
+        v[4 * i + 2] = __uint_as_float(r[4 * i + 2]) + b4.z;
+        v[4 * i + 3] = __uint_as_float(r[4 * i + 3]) + b4.w;
+    }
+    if (p.ep.act == QMM_ACT_GELU_TANH) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const float2 t = activate<true>(make_float2(v[i], v[i + 1]));
+            v[i] = t.x, v[i + 1] = t.y;
+        }
+    } else if (p.ep.act == QMM_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const float2 t = activate<false>(make_float2(v[i], v[i + 1]));
+            v[i] = t.x, v[i + 1] = t.y;
+        }
+    }
+    if (p.ep.gate) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 g4 = gate[i];
+            v[4 * i] *= g4.x;
+            v[4 * i + 1] *= g4.y;
+            v[4 * i + 2] *= g4.z;
+            v[4 * i + 3] *= g4.w;
+        }
+    }
+    auto cell = [&](int g) { return reinterpret_cast<uint4 *>(o.stage + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)); };
+    if (p.ep.residual) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {  // eight features: 16 bytes of this token's row
+            float res[8];
+            if (res_tma) {
+                Vec8<Bf16> w;
+                w.w[0] = *cell(g);
+                vec8_to_f32(w, res);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int f = f0 + g * 8 + e;
+                    res[e] = row < p.m && f < p.n ? bf16_bits_to_f32(p.ep.residual[(int64_t)row * p.n + f]) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[g * 8 + e] = p.ep.res_mul ? res[e] * v[g * 8 + e] : res[e] + v[g * 8 + e];
+        }
+    }
+    if (!res_tma) {
+        if (lane == 0) bulk_wait_read<0>();  // the last store has left the buffer
+        __syncwarp();
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+        *cell(g) = make_uint4(pack_bf16x2_rn(v[8 * g], v[8 * g + 1]), pack_bf16x2_rn(v[8 * g + 2], v[8 * g + 3]),
+                              pack_bf16x2_rn(v[8 * g + 4], v[8 * g + 5]), pack_bf16x2_rn(v[8 * g + 6], v[8 * g + 7]));
+    if (p.tma_out) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(tmap_y, o.stage, f0, m0);
+            bulk_commit();
+        }
+    } else {
+        __syncwarp();
+        const int rows = min(32, p.m - m0);
+        for (int t = 0; t < rows; ++t) {
+            const uint16_t w = *reinterpret_cast<const uint16_t *>(o.stage + t * 64 + (((lane >> 3) ^ ((t >> 1) & 3)) << 4) + (lane & 7) * 2);
+            if (f0 + lane < p.n) p.y[(int64_t)(m0 + t) * p.n + f0 + lane] = w;
+        }
+        __syncwarp();
+    }
+}
+
+// A tile's chunks of one warp.  feature(c): the c-th chunk's first feature (p.n or more: none); column(c): its accumulator
+// column; loaded(c) runs once chunk c is in registers; q counts the warp's chunks so far.  False: a wait ran out.
+template <bool CLUSTER, typename Feature, typename Column, typename Loaded>
+__device__ __forceinline__ bool tile_epilogue(const Params &p, const CUtensorMap *tmap_y, const CUtensorMap *tmap_res, const ChunkOut &o, uint64_t *acc_full,
+                                              uint32_t parity, uint32_t tmem, int m0, uint32_t &q, const Feature &feature, const Column &column,
+                                              const Loaded &loaded) {
+    const int lane = threadIdx.x & 31;
+    const bool res_tma = p.tma_out && p.ep.residual;
+    // A quadrant past the last token or a chunk past the last feature has nothing to store.
+    auto live = [&](int c) { return m0 < p.m && feature(c) < p.n; };
+    bool requested = res_tma && live(0);
+    if (requested) request_residual(tmap_res, o, feature(0), m0);
+    {
+        FeatureConsts fc[kMaxChunks];
+#pragma unroll
+        for (int c = 0; c < kMaxChunks; ++c) fc[c] = load_feature_consts(p.ep, feature(c) + lane, feature(c) + lane < p.n);
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < kMaxChunks; ++c) {
+            o.vec[c * 2 * kChunk + lane] = fc[c].bias;
+            o.vec[c * 2 * kChunk + kChunk + lane] = fc[c].gate;
+        }
+        __syncwarp();
+    }
+    if (!__all_sync(0xffffffffu, mbar_wait<CLUSTER>(acc_full, parity, p.err, kErrTimeoutEpilogue))) {
+        if (requested) mbar_wait(o.res_full, q & 1, p.err, kErrTimeoutDrain);
+        return false;
+    }
+    tc_fence_after_sync();
+#pragma unroll
+    for (int c = 0; c < kMaxChunks; ++c) {
+        uint32_t r[32];
+        if (live(c)) {
+            tmem_ld_32x32b_x32(tmem + column(c), r);
+            if (res_tma && !requested) request_residual(tmap_res, o, feature(c), m0);
+            tc_wait_ld();
+        }
+        loaded(c);
+        if (live(c)) {
+            if (res_tma && !__all_sync(0xffffffffu, mbar_wait(o.res_full, q & 1, p.err, kErrTimeoutEpilogue))) return false;
+            chunk_finish(p, tmap_y, o, o.vec + c * 2 * kChunk, r, feature(c), m0, res_tma);
+            requested = false;
+            ++q;
+        }
+    }
+    return true;
+}
+
 template <int TN>
 __global__ void __launch_bounds__(kThreads, 1)
     mx4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
@@ -115,8 +301,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *acc_full = empty + S;                                    // [2]
     uint64_t *acc_empty = acc_full + 2;                                // [2]
     uint64_t *drain = acc_empty + 2;
-    uint64_t *res_full = drain + 1;                                    // [warp][2] residual chunk landed
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_full + kEpiWarps * 2);
+    uint64_t *res_full = drain + 1;                                    // [warp] residual chunk landed
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_full + kEpiWarps);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -129,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&acc_empty[b], kEpiWarps);
         }
         mbar_init(drain, 1);
-        for (int i = 0; i < kEpiWarps * 2; ++i) mbar_init(&res_full[i], 1);
+        for (int i = 0; i < kEpiWarps; ++i) mbar_init(&res_full[i], 1);
         fence_barrier_init();
     }
     if (warp == kMma) {
@@ -154,7 +340,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t i = 0;
         bool ok = true;
         for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-            const int m0 = t % p.m_tiles * kTM, n0 = t / p.m_tiles * TN;
+            int mt, nt;
+            tile_at(p, t, mt, nt);
+            const int m0 = mt * kTM, n0 = nt * TN;
             const int rt = n0 >> 7;
             const int nbt = min(C::kBTiles, p.b_row_tiles - rt);  // (TN and a start inside a tile fit kBTiles tiles)
             for (int kb = 0; kb < p.nkb; ++kb, ++i) {
@@ -189,7 +377,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t adesc0 = sdesc_kmajor_sw128(smem_u32(smem + C::kAOff)), bdesc0 = sdesc_kmajor_sw128(smem_u32(smem + C::kBOff));
         const uint64_t sadesc0 = sdesc_scales(smem_u32(smem + C::kSfaOff)), sbdesc0 = sdesc_scales(smem_u32(smem + C::kSfbOff));
         for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++lt) {
-            const int n0 = t / p.m_tiles * TN;
+            int mt, nt;
+            tile_at(p, t, mt, nt);
+            const int n0 = nt * TN;
             const int rt = n0 >> 7;
             const int nbt = min(C::kBTiles, p.b_row_tiles - rt);
             const uint32_t shift = (uint32_t)(n0 & 127) >> 5;  // columns into the first scale tile
@@ -237,106 +427,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         // ------------------------------------------------------------ epilogue
         pdl_dependency_wait();
-        const int quad = warp & 3, half = warp >> 2;
-        constexpr int kChunks = TN / 2 / kChunk;  // chunks of this warp's half
-        uint8_t *const out = smem + C::kOutOff + warp * 2 * kChunk * 64;
-        float *const vec = reinterpret_cast<float *>(smem + C::kVecOff) + warp * 2 * kChunk;
-        uint64_t *const rbar = res_full + warp * 2;
-        const bool res_tma = p.tma_out && p.ep.residual;
-        uint32_t q = 0;  // chunks so far
+        const int quad = warp & 3, group = warp >> 2;
+        const ChunkOut o{smem + C::kOutOff + warp * kChunk * 64, reinterpret_cast<float *>(smem + C::kVecOff) + warp * kMaxChunks * 2 * kChunk,
+                         res_full + warp};
+        uint32_t q = 0;
         int lt = 0;
         for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++lt) {
-            const int m0 = t % p.m_tiles * kTM + quad * 32, n0 = t / p.m_tiles * TN + half * (TN / 2);
-            const int row = m0 + lane;
+            int mt, nt;
+            tile_at(p, t, mt, nt);
+            const int m0 = mt * kTM + quad * 32, n0 = nt * TN;
             const int b = lt & 1;
-            // A quadrant past the last token or a chunk past the last feature has nothing to store.
-            const int chunks = m0 < p.m ? min(kChunks, (p.n - n0 + kChunk - 1) / kChunk) : 0;
-            auto load_residual = [&](int c, uint32_t buf) {
-                if (lane == 0) {
-                    bulk_wait_read<0>();  // stores from this buffer have left it
-                    mbar_arrive_expect_tx(&rbar[buf], kChunk * 64);
-                    tma_load_2d(out + buf * kChunk * 64, &tmap_res, &rbar[buf], n0 + c * kChunk, m0);
-                }
-            };
-            if (res_tma && chunks > 0) load_residual(0, q & 1);
-            if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[b], (lt >> 1) & 1, p.err, kErrTimeoutEpilogue))) {
-                if (res_tma && chunks > 0) mbar_wait(&rbar[q & 1], (q >> 1) & 1, p.err, kErrTimeoutDrain);
-                break;
-            }
-            tc_fence_after_sync();
-            bool ok = true;
-            for (int c = 0; c < chunks; ++c, ++q) {
-                const uint32_t buf = q & 1;
-                uint8_t *const o = out + buf * kChunk * 64;
-                const int f0 = n0 + c * kChunk;
-                uint32_t r[32];
-                tmem_ld_32x32b_x32(tmem + ((uint32_t)(quad * 32) << 16) + b * TN + half * (TN / 2) + c * kChunk, r);
-                if (res_tma) {
-                    if (c + 1 < chunks) load_residual(c + 1, buf ^ 1);
-                } else if (lane == 0) {
-                    bulk_wait_read<1>();
-                }
-                {
-                    const FeatureConsts fc = load_feature_consts(p.ep, f0 + lane, f0 + lane < p.n);
-                    __syncwarp();
-                    vec[lane] = fc.bias;
-                    vec[kChunk + lane] = fc.gate;
-                    __syncwarp();
-                }
-                if (res_tma) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&rbar[buf], (q >> 1) & 1, p.err, kErrTimeoutEpilogue));
-                    if (!ok) {
-                        if (c + 1 < chunks) mbar_wait(&rbar[buf ^ 1], ((q + 1) >> 1) & 1, p.err, kErrTimeoutDrain);
-                        break;
-                    }
-                }
-                tc_wait_ld();
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {  // eight features: 16 bytes of this token's row
-                    uint4 *const cell = reinterpret_cast<uint4 *>(o + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4));
-                    float v[8], res[8];
-                    if (p.ep.residual) {
-                        if (res_tma) {
-                            Vec8<Bf16> w;
-                            w.w[0] = *cell;
-                            vec8_to_f32(w, res);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const int f = f0 + g * 8 + e;
-                                res[e] = row < p.m && f < p.n ? bf16_bits_to_f32(p.ep.residual[(int64_t)row * p.n + f]) : 0.0f;
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const FeatureConsts fc{vec[g * 8 + e], vec[kChunk + g * 8 + e]};
-                        v[e] = epilogue_value_rv(p.ep, fc, __uint_as_float(r[g * 8 + e]), p.ep.residual ? res[e] : 0.0f);
-                    }
-                    *cell = make_uint4(pack_bf16x2_rn(v[0], v[1]), pack_bf16x2_rn(v[2], v[3]), pack_bf16x2_rn(v[4], v[5]),
-                                       pack_bf16x2_rn(v[6], v[7]));
-                }
-                if (p.tma_out) {
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) {
-                        tma_store_2d(&tmap_y, o, f0, m0);
-                        bulk_commit();
-                    }
-                } else {
-                    __syncwarp();
-                    const int rows = min(32, p.m - m0);
-                    for (int rr = 0; rr < rows; ++rr) {
-                        const uint16_t v = *reinterpret_cast<const uint16_t *>(o + rr * 64 + (((lane >> 3) ^ ((rr >> 1) & 3)) << 4) + (lane & 7) * 2);
-                        if (f0 + lane < p.n) p.y[(int64_t)(m0 + rr) * p.n + f0 + lane] = v;
-                    }
-                }
+            auto place = [&](int c) { return kChunk * (kGroups * c + group); };
+            auto feature = [&](int c) { return place(c) < TN ? n0 + place(c) : INT_MAX - kChunk; };
+            auto column = [&](int c) { return ((uint32_t)(quad * 32) << 16) + b * TN + place(c); };
+            auto loaded = [&](int c) {
+                if (c + 1 < kMaxChunks) return;
+                tc_fence_before_sync();
                 __syncwarp();
-            }
-            if (!ok) break;
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[b]);
+                if (lane == 0) mbar_arrive(&acc_empty[b]);
+            };
+            if (!tile_epilogue<false>(p, &tmap_y, &tmap_res, o, &acc_full[b], (lt >> 1) & 1, tmem, m0, q, feature, column, loaded)) break;
         }
         if (lane == 0) bulk_wait_all();
     }
@@ -345,6 +455,245 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kMma) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
+    }
+}
+
+// ------------------------------------------------------------------- CTA pairs
+// The same product on pairs of CTAs (cta_group::2): a tile of 256 tokens x 256
+// features, each CTA holding 128 tokens and half of the features in its shared
+// memory and accumulating its tokens for all of them.  Against the 128 x 192 tile
+// of one CTA this reads 35 KB instead of 43 KB of operands for 1.33 times the
+// work, and spreads six scale copies over it.  B200, back to back: 4352 x 12288 x
+// 3072 74 us (4.45 PFLOP/s; one-CTA tiles 90), 16384 x 3072 x 12288 323 us, with GELU
+// 340 (369, 459).  Without its loads the first runs in 58 us, without its epilogue
+// in 68, without both in 54: operands out of L2 and the power they cost bound it.
+//
+// Two accumulators of 256 columns and a scale slot for each stage do not fit the
+// 512 columns of tensor memory, so the accumulators share 120 columns: [0, 256) and
+// [136, 392).  The epilogue takes the half of a tile that holds them first, and the
+// next tile's main loop starts once it is in registers.
+struct PairCfg {
+    static constexpr int kTN = 256;
+    static constexpr int kABytes = kTM * kRowBytes;
+    static constexpr int kBBytes = kTN / 2 * kRowBytes;
+    static constexpr int kSfaBytes = 2 * kSfTile, kSfbBytes = 4 * kSfTile;
+    static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
+    static constexpr int kOutBytes = kEpiWarps * kChunk * 64;
+    static constexpr int kVecBytes = kEpiWarps * kMaxChunks * 2 * kChunk * 4;
+    static constexpr int kStages = 5;
+    static constexpr int kSfCols = 24;
+    static constexpr int kAcc1 = 512 - kStages * kSfCols - kTN;  // 136
+    static constexpr int kSfCol0 = kAcc1 + kTN;                  // 392
+    static_assert(kAcc1 >= kTN / 2, "the halves drained first hold every shared column");
+    static constexpr int kAOff = 0;
+    static constexpr int kBOff = kAOff + kStages * kABytes;
+    static constexpr int kOutOff = kBOff + kStages * kBBytes;
+    static constexpr int kSfaOff = kOutOff + kOutBytes;
+    static constexpr int kSfbOff = kSfaOff + kStages * kSfaBytes;
+    static constexpr int kVecOff = kSfbOff + kStages * kSfbBytes;
+    static constexpr int kBarOff = kVecOff + kVecBytes;
+    static constexpr int kNumBars = 2 * kStages + 4 + 1 + 1 + kEpiWarps;
+    static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
+    static_assert(kSmemBytes <= 232448, "shared memory");
+    static constexpr uint32_t kIdesc = (1u << 7) | (1u << 10) | ((uint32_t)(kTN >> 3) << 17) | (1u << 23) | ((uint32_t)(2 * kTM >> 4) << 24);
+};
+
+__device__ __forceinline__ void tc_copy_scales_pair(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+__device__ __forceinline__ void tc_mma_mxf4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                                 uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+// 3-D tiled load by either CTA of a pair, completion counted on a barrier of either (no multicast).
+__device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *map, uint32_t bar_cluster, int32_t c0, int32_t c1, int32_t c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+
+__global__ void __launch_bounds__(kThreads, 1)
+    mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                         const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb,
+                         const __grid_constant__ CUtensorMap tmap_y, const __grid_constant__ CUtensorMap tmap_res, const Params p) {
+    using C = PairCfg;
+    constexpr int S = C::kStages, TN = C::kTN;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::kBarOff);  // [S] leader: both CTAs' stage landed
+    uint64_t *empty = full + S;                                        // [S] stage's MMAs complete (both CTAs)
+    uint64_t *acc_full = empty + S;                                    // [2] (both CTAs)
+    uint64_t *acc_empty = acc_full + 2;                                // [2] leader: drained by both CTAs
+    uint64_t *shared_cols = acc_empty + 2;                             // leader: a tile's shared columns are in registers
+    uint64_t *drain = shared_cols + 1;
+    uint64_t *res_full = drain + 1;                                    // [warp] residual chunk landed
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_full + kEpiWarps);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int unit = (int)cluster_id_x(), units = (int)cluster_count_x();
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&acc_full[b], 1);
+            mbar_init(&acc_empty[b], 2 * kEpiWarps);
+        }
+        mbar_init(shared_cols, 2 * kEpiWarps);
+        mbar_init(drain, 1);
+        for (int i = 0; i < kEpiWarps; ++i) mbar_init(&res_full[i], 1);
+        fence_barrier_init();
+    }
+    if (warp == kMma) {
+        tmem_alloc_pair(tmem_slot, 512);
+        tmem_relinquish_pair();
+    }
+    if (warp == kProducer && lane == 0) {
+        tma_prefetch_desc(&tmap_a);
+        tma_prefetch_desc(&tmap_b);
+        tma_prefetch_desc(&tmap_sfa);
+        tma_prefetch_desc(&tmap_sfb);
+        if (p.tma_out) tma_prefetch_desc(&tmap_y);
+        if (p.tma_out && p.ep.residual) tma_prefetch_desc(&tmap_res);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync();  // barriers initialised and tensor memory allocated in both CTAs
+    tc_fence_after_sync();
+    const uint32_t tmem = *tmem_slot;
+    const int tiles = p.m_tiles * p.n_tiles;
+
+    if (warp == kProducer) {
+        // ------------------------------------------------------------ producer
+        pdl_dependency_wait();
+        uint32_t i = 0;
+        bool ok = true;
+        for (int t = unit; ok && t < tiles; t += units) {
+            int mt, nt;
+            tile_at(p, t, mt, nt);
+            const int m0 = mt * (2 * kTM) + (int)rank * kTM, n0 = nt * TN;
+            for (int kb = 0; kb < p.nkb; ++kb, ++i) {
+                const int s = i % S;
+                if (!mbar_wait<true>(&empty[s], ((i / S) & 1) ^ 1, p.err, kErrTimeoutProducer)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) {
+                    const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+                    if (leader) mbar_arrive_expect_tx(&full[s], 2 * C::kStageBytes);
+                    tma_load_2d_pair(smem + C::kAOff + s * C::kABytes, &tmap_a, bar, kb * kRowBytes, m0);
+                    tma_load_2d_pair(smem + C::kBOff + s * C::kBBytes, &tmap_b, bar, kb * kRowBytes, n0 + (int)rank * (TN / 2));
+                    tma_load_3d_pair(smem + C::kSfaOff + s * C::kSfaBytes, &tmap_sfa, bar, 0, kb * 4, m0 >> 7);
+                    tma_load_3d_pair(smem + C::kSfbOff + s * C::kSfbBytes, &tmap_sfb, bar, 0, kb * 4, n0 >> 7);
+                }
+                __syncwarp();
+            }
+        }
+        pdl_launch_dependents();
+        if (!ok && leader) {  // let the pair's copies already issued land before either CTA exits
+            const uint32_t first = i > (uint32_t)S ? i - S : 0;
+            for (uint32_t j = first; j < i; ++j) mbar_wait<true>(&full[j % S], (j / S) & 1, p.err, kErrTimeoutDrain);
+        }
+    } else if (warp == kMma) {
+        // ------------------------------------------------------------ MMA issuer
+        if (leader) {
+            bool ok = true, issued = false;
+            uint32_t i = 0;
+            int lt = 0;
+            constexpr uint16_t kBoth = 0x3;
+            const uint64_t adesc0 = sdesc_kmajor_sw128(smem_u32(smem + C::kAOff)), bdesc0 = sdesc_kmajor_sw128(smem_u32(smem + C::kBOff));
+            const uint64_t sadesc0 = sdesc_scales(smem_u32(smem + C::kSfaOff)), sbdesc0 = sdesc_scales(smem_u32(smem + C::kSfbOff));
+            for (int t = unit; ok && t < tiles; t += units, ++lt) {
+                const int b = lt & 1;
+                ok = mbar_wait<true>(&acc_empty[b], ((lt >> 1) & 1) ^ 1, p.err, kErrTimeoutMma);
+                if (ok && lt > 0) ok = mbar_wait<true>(shared_cols, (lt - 1) & 1, p.err, kErrTimeoutMma);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t d = tmem + (b ? C::kAcc1 : 0);
+                uint32_t acc = 0;
+                for (int kb = 0; kb < p.nkb; ++kb, ++i) {
+                    const uint32_t s = i % S;
+                    ok = mbar_wait<true>(&full[s], (i / S) & 1, p.err, kErrTimeoutMma);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    if (lane_elect()) {
+                        const uint32_t sfa = tmem + C::kSfCol0 + s * C::kSfCols, sfb = sfa + 8;
+                        const uint64_t ad = adesc0 + (uint64_t)s * (C::kABytes >> 4), bd = bdesc0 + (uint64_t)s * (C::kBBytes >> 4);
+                        const uint64_t sad = sadesc0 + (uint64_t)s * (C::kSfaBytes >> 4), sbd = sbdesc0 + (uint64_t)s * (C::kSfbBytes >> 4);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {  // 128 columns: one scale tile along k
+                            tc_copy_scales_pair(sfa + h * 4, sad + h * (kSfTile >> 4));
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) tc_copy_scales_pair(sfb + h * 8 + j * 4, sbd + (j * 2 + h) * (kSfTile >> 4));
+                        }
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            const uint32_t id = (kk & 1) * 2;  // which two of the cell's four scales
+                            tc_mma_mxf4_pair(d, ad + kk * 2, bd + kk * 2, C::kIdesc | (id << 4) | (id << 29), sfa + (kk >> 1) * 4,
+                                             sfb + (kk >> 1) * 8, acc);
+                            acc = 1;
+                        }
+                        tc_commit_pair_multicast(&empty[s], kBoth);
+                    }
+                    acc = 1;
+                    issued = true;
+                }
+                if (!ok) break;
+                if (lane_elect()) tc_commit_pair_multicast(&acc_full[b], kBoth);
+                __syncwarp();
+            }
+            if (!ok && issued) {
+                if (lane_elect()) tc_commit_pair_multicast(drain, 0x1);
+                __syncwarp();
+                mbar_wait<true>(drain, 0, p.err, kErrTimeoutDrain);
+            }
+        }
+    } else {
+        // ------------------------------------------------------------ epilogue
+        pdl_dependency_wait();
+        const int quad = warp & 3, group = warp >> 2;
+        const ChunkOut o{smem + C::kOutOff + warp * kChunk * 64, reinterpret_cast<float *>(smem + C::kVecOff) + warp * kMaxChunks * 2 * kChunk,
+                         res_full + warp};
+        uint32_t q = 0;
+        int lt = 0;
+        for (int t = unit; t < tiles; t += units, ++lt) {
+            int mt, nt;
+            tile_at(p, t, mt, nt);
+            const int m0 = mt * (2 * kTM) + (int)rank * kTM + quad * 32, n0 = nt * TN;
+            const int b = lt & 1;
+            // The upper half first in the first accumulator, the lower half in the second: the shared columns are among them.
+            auto place = [&](int c) { return kChunk * (kGroups * (b ? c : 1 - c) + group); };
+            auto feature = [&](int c) { return n0 + place(c); };
+            auto column = [&](int c) { return ((uint32_t)(quad * 32) << 16) + (b ? C::kAcc1 : 0) + place(c); };
+            auto loaded = [&](int c) {
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(c == 0 ? shared_cols : &acc_empty[b]), 0));
+            };
+            if (!tile_epilogue<true>(p, &tmap_y, &tmap_res, o, &acc_full[b], (lt >> 1) & 1, tmem, m0, q, feature, column, loaded)) break;
+        }
+        if (lane == 0) bulk_wait_all();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    cluster_sync();  // the peer's arrivals, copies and MMAs on this CTA are over
+    if (warp == kMma) {
+        tc_fence_after_sync();
+        tmem_dealloc_pair(tmem, 512);
     }
 }
 
@@ -378,35 +727,56 @@ static qmm_status map_2d(CUtensorMap *map, CUtensorMapDataType type, const void 
     return QMM_OK;
 }
 
-template <int TN>
-static qmm_status launch_gemm(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epilogue &ep, uint16_t *y, cudaStream_t st) {
-    using C = Cfg<TN>;
-    auto kernel = mx4_gemm_kernel<TN>;
-    static bool configured[64] = {};
+// Scales as [row tiles][256-byte rows]: a stage's two tiles of a row tile are four consecutive rows.
+static qmm_status map_scales(CUtensorMap *map, const uint8_t *scales, int64_t rows, int64_t k, uint32_t row_tiles_a_box) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(QMM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t per = (cuuint64_t)mx4_scale_tiles(k) * 2;
+    cuuint64_t dims[3] = {256, per, (cuuint64_t)mx4_row_tiles(rows)};
+    cuuint64_t strides[2] = {256, per * 256};
+    cuuint32_t box[3] = {256, 4, row_tiles_a_box};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(scales), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(QMM_ERR_CUDA, "cuTensorMapEncodeTiled (scales) failed (%d)", (int)r);
+    return QMM_OK;
+}
+
+template <typename K>
+static qmm_status allow_smem(K kernel, int bytes, bool (&configured)[64]) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) dev = 0;
     if (!configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != cudaSuccess) return cuda_fail(e, "mxfp4 gemm smem attribute");
         configured[dev] = true;
     }
+    return QMM_OK;
+}
+
+// Tensor maps of the operands and output, and what both kernels need to know.
+struct Problem {
+    CUtensorMap a, b, y, res;
+    Params p;
+};
+
+static qmm_status make_problem(Problem &q, const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epilogue &ep, uint16_t *y, int tm, int tn, int b_rows) {
     const uint64_t pitch = (uint64_t)mx4_pitch(w.k);
-    CUtensorMap ta, tb, ty, tr;
-    qmm_status s = map_2d(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, x.codes, pitch, (uint64_t)x.rows, pitch, kRowBytes, kTM, CU_TENSOR_MAP_SWIZZLE_128B);
+    qmm_status s = map_2d(&q.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, x.codes, pitch, (uint64_t)x.rows, pitch, kRowBytes, kTM, CU_TENSOR_MAP_SWIZZLE_128B);
     if (s != QMM_OK) return s;
-    s = map_2d(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes, pitch, (uint64_t)w.rows, pitch, kRowBytes, TN, CU_TENSOR_MAP_SWIZZLE_128B);
+    s = map_2d(&q.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes, pitch, (uint64_t)w.rows, pitch, kRowBytes, (uint32_t)b_rows, CU_TENSOR_MAP_SWIZZLE_128B);
     if (s != QMM_OK) return s;
     const bool tma_out = w.rows % 8 == 0;  // rows of y on 16-byte boundaries
-    ty = tr = ta;
+    q.y = q.res = q.a;
     if (tma_out) {
-        s = map_2d(&ty, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, y, (uint64_t)w.rows, (uint64_t)x.rows, (uint64_t)w.rows * 2, kChunk, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+        s = map_2d(&q.y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, y, (uint64_t)w.rows, (uint64_t)x.rows, (uint64_t)w.rows * 2, kChunk, 32, CU_TENSOR_MAP_SWIZZLE_64B);
         if (s == QMM_OK && ep.residual)
-            s = map_2d(&tr, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ep.residual, (uint64_t)w.rows, (uint64_t)x.rows, (uint64_t)w.rows * 2, kChunk, 32,
+            s = map_2d(&q.res, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ep.residual, (uint64_t)w.rows, (uint64_t)x.rows, (uint64_t)w.rows * 2, kChunk, 32,
                        CU_TENSOR_MAP_SWIZZLE_64B);
         if (s != QMM_OK) return s;
     }
-    Params p;
+    Params &p = q.p;
     p.a_scales = x.scales;
     p.b_scales = w.scales;
     p.ep = epilogue_args(ep);
@@ -415,18 +785,68 @@ static qmm_status launch_gemm(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epil
     p.n = (int32_t)w.rows;
     p.nkb = (int32_t)((w.k + kBK - 1) / kBK);
     p.sf_tiles = (int32_t)mx4_scale_tiles(w.k);
-    p.m_tiles = (int32_t)((x.rows + kTM - 1) / kTM);
-    p.n_tiles = (int32_t)((w.rows + TN - 1) / TN);
+    const int64_t mt = (x.rows + tm - 1) / tm, nt = (w.rows + tn - 1) / tn;
+    if (mt * nt > INT32_MAX / 2) return fail(QMM_ERR_UNSUPPORTED, "mxfp4 linear: too many output tiles");
+    p.m_tiles = (int32_t)mt;
+    p.n_tiles = (int32_t)nt;
     p.b_row_tiles = (int32_t)mx4_row_tiles(w.rows);
     p.tma_out = tma_out ? 1 : 0;
     p.err = device_error_word();
-    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
-    if (tiles > INT32_MAX / 2) return fail(QMM_ERR_UNSUPPORTED, "mxfp4 linear: too many output tiles");
-    const unsigned grid = (unsigned)std::min<int64_t>(tiles, sm_count());
-    kernel<<<grid, kThreads, C::kSmemBytes, st>>>(ta, tb, ty, tr, p);
+    return QMM_OK;
+}
+
+template <int TN>
+static qmm_status launch_gemm(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epilogue &ep, uint16_t *y, cudaStream_t st) {
+    using C = Cfg<TN>;
+    static bool configured[64] = {};
+    qmm_status s = allow_smem(mx4_gemm_kernel<TN>, C::kSmemBytes, configured);
+    if (s != QMM_OK) return s;
+    Problem q;
+    s = make_problem(q, w, x, ep, y, kTM, TN, TN);
+    if (s != QMM_OK) return s;
+    const unsigned grid = (unsigned)std::min<int64_t>((int64_t)q.p.m_tiles * q.p.n_tiles, sm_count());
+    mx4_gemm_kernel<TN><<<grid, kThreads, C::kSmemBytes, st>>>(q.a, q.b, q.y, q.res, q.p);
     count_launch();
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? QMM_OK : cuda_fail(e, "mxfp4 gemm launch");
+}
+
+static qmm_status launch_gemm_pair(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epilogue &ep, uint16_t *y, cudaStream_t st) {
+    using C = PairCfg;
+    static bool configured[64] = {};
+    qmm_status s = allow_smem(mx4_gemm_pair_kernel, C::kSmemBytes, configured);
+    if (s != QMM_OK) return s;
+    Problem q;
+    s = make_problem(q, w, x, ep, y, 2 * kTM, C::kTN, C::kTN / 2);
+    if (s != QMM_OK) return s;
+    CUtensorMap sfa, sfb;
+    if ((s = map_scales(&sfa, x.scales, x.rows, x.k, 1)) != QMM_OK) return s;
+    if ((s = map_scales(&sfb, w.scales, w.rows, w.k, 2)) != QMM_OK) return s;
+    const unsigned pairs = (unsigned)std::min<int64_t>((int64_t)q.p.m_tiles * q.p.n_tiles, std::max(1, sm_count() / 2));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(pairs * 2, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, mx4_gemm_pair_kernel, q.a, q.b, sfa, sfb, q.y, q.res, q.p);
+    count_launch();
+    if (e == cudaSuccess) e = cudaGetLastError();
+    return e == cudaSuccess ? QMM_OK : cuda_fail(e, "mxfp4 gemm launch");
+}
+
+// Pairs where their 256 x 256 tiles fill at least half of the SM pairs; below
+// that the 128 x 192 tiles keep more SMs busy.
+static qmm_status launch_product(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epilogue &ep, uint16_t *y, cudaStream_t st) {
+    const int64_t pair_tiles = ((x.rows + 255) / 256) * ((w.rows + 255) / 256);
+    if (pair_tiles * 4 >= sm_count()) return launch_gemm_pair(w, x, ep, y, st);
+    return launch_gemm<192>(w, x, ep, y, st);
 }
 
 }  // namespace mx4
@@ -507,7 +927,7 @@ qmm_status qmm_mx4_linear(const qmm_mx4_linear_args *p, void *stream) {
         if (s != QMM_OK) return s;
     }
     const qmm_epilogue ep{a.bias, a.gate, a.residual, a.activation};
-    return qmm::mx4::launch_gemm<192>(a.w, x, ep, a.y, st);
+    return qmm::mx4::launch_product(a.w, x, ep, a.y, st);
 }
 
 }  // extern "C"
