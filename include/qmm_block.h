@@ -78,8 +78,10 @@ QMM_API qmm_status qmm_mx4_row_scales(const uint8_t *scales, int64_t rows, int64
  * residual * (gate * act(...)) with QMM_EPILOGUE_RESIDUAL_MUL, one rounding to
  * bf16; W [n, k] MXFP4.  x is either MXFP4 (x_codes and x_scales; x NULL) or a
  * matrix of bf16, f32 or f16 (x, x_elem, x_row_stride), which is first
- * quantised by the rule of qmm_mx4_quantize into `workspace`
- * (qmm_mx4_workspace_bytes(m, k) bytes, 16-byte aligned).  Products of codes
+ * quantised by the rule of qmm_mx4_quantize, within the product where m is
+ * small, else into `workspace` (16-byte aligned,
+ * qmm_mx4_linear_workspace_bytes(m, n, k) bytes: 0 in the former case, never
+ * more than qmm_mx4_workspace_bytes(m, k)).  Products of codes
  * and scales are exact, sums are f32.  bias, gate bf16 [n] or NULL; residual
  * bf16 [m, n] or NULL, it may alias y.  y must not overlap x, W or workspace.
  * Calls that share a workspace must be ordered on one stream.
@@ -102,6 +104,7 @@ typedef struct qmm_mx4_linear_args {
 } qmm_mx4_linear_args;
 
 QMM_API uint64_t qmm_mx4_workspace_bytes(int64_t m, int64_t k);
+QMM_API uint64_t qmm_mx4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
 QMM_API qmm_status qmm_mx4_linear(const qmm_mx4_linear_args *a, void *stream);
 
 /* ----------------------------------------------------------------- rotary */

@@ -128,6 +128,7 @@ extern "C" {
         scales: *const u8, rows: i64, k: i64, row_major: *mut u8, stream: *mut c_void,
     ) -> qmm_status;
     pub fn qmm_mx4_workspace_bytes(m: i64, k: i64) -> u64;
+    pub fn qmm_mx4_linear_workspace_bytes(m: i64, n: i64, k: i64) -> u64;
     pub fn qmm_mx4_linear(a: *const qmm_mx4_linear_args, stream: *mut c_void) -> qmm_status;
     pub fn qmm_qk_norm_rotary(a: *const qmm_rotary_args, stream: *mut c_void) -> qmm_status;
     pub fn qmm_gated_residual_norm(a: *const qmm_gated_norm_args, stream: *mut c_void) -> qmm_status;

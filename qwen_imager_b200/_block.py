@@ -29,6 +29,7 @@ EXPORTED_SYMBOLS = (
     "qmm_mx4_tile_scales",
     "qmm_mx4_row_scales",
     "qmm_mx4_workspace_bytes",
+    "qmm_mx4_linear_workspace_bytes",
     "qmm_mx4_linear",
     "qmm_qk_norm_rotary",
     "qmm_gated_residual_norm",
@@ -52,6 +53,7 @@ def load() -> ctypes.CDLL:
                 ("qmm_mx4_code_bytes", ctypes.c_uint64, [i64, i64]),
                 ("qmm_mx4_scale_bytes", ctypes.c_uint64, [i64, i64]),
                 ("qmm_mx4_workspace_bytes", ctypes.c_uint64, [i64, i64]),
+                ("qmm_mx4_linear_workspace_bytes", ctypes.c_uint64, [i64, i64, i64]),
                 ("qmm_mx4_quantize", i32, [vp, i32, i64, i64, i64, vp, vp, vp]),
                 ("qmm_mx4_dequantize", i32, [args, vp, i32, vp]),
                 ("qmm_mx4_tile_scales", i32, [vp, i64, i64, vp, vp]),

@@ -22,19 +22,13 @@
 // means that the MMAs that read its slot are complete.  Every wait is bounded.
 #include <algorithm>
 #include <climits>
-#include <mutex>
 
-#include "qmm_epilogue.cuh"
-#include "qmm_internal.h"
-#include "qmm_mx4.cuh"
+#include "qmm_mx4_mma.cuh"
 
 namespace qmm {
 namespace mx4 {
 
 constexpr int kTM = 128;         // tokens a tile
-constexpr int kBK = 256;         // columns a stage
-constexpr int kRowBytes = 128;   // codes of a row in a stage
-constexpr int kSfTile = 512;     // scales of 128 rows x 4 blocks
 constexpr int kEpiWarps = 16;
 constexpr int kProducer = kEpiWarps, kMma = kEpiWarps + 1;
 constexpr int kThreads = (kEpiWarps + 2) * 32;
@@ -68,8 +62,7 @@ struct Cfg {
     static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
     static constexpr int kSfCol0 = 2 * TN;
     static_assert(kStages >= 2 && kSmemBytes <= 232448, "shared memory");
-    // kind::mxf4 instruction descriptor: E2M1 operands, UE8M0 scales, M = 128, N = TN.
-    static constexpr uint32_t kIdesc = (1u << 7) | (1u << 10) | ((uint32_t)(TN >> 3) << 17) | (1u << 23) | ((uint32_t)(kTM >> 4) << 24);
+    static constexpr uint32_t kIdesc = idesc_mxf4(kTM, TN);
 };
 
 struct Params {
@@ -88,56 +81,6 @@ struct Params {
 __device__ __forceinline__ void tile_at(const Params &p, int t, int &mt, int &nt) {
     nt = t / p.m_tiles;
     mt = t - nt * p.m_tiles;
-}
-
-// Shared-memory descriptor of a 512-byte scale tile (32 rows of 16 bytes, no
-// swizzle: 8-row groups 128 bytes apart).
-__device__ __forceinline__ uint64_t sdesc_scales(uint32_t smem_addr) {
-    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(128u >> 4) << 32) | ((uint64_t)1u << 46);
-}
-
-// 32 rows x 128 bits into four tensor-memory columns, repeated in the four lane quadrants.
-__device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-
-__device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                            uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-}
-
-// t * sigmoid(z) of two values: both activations in one exponential and one
-// reciprocal a value (GELU's 0.5 (1 + tanh u) is sigmoid(2 u)).  The fast forms are
-// good to a few 2^-22 of the result, far below its rounding to bf16; past their range
-// they give 0 or t.
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float rcp_fast(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-template <bool GELU>
-__device__ __forceinline__ float2 activate(float2 t) {
-    const float2 zero = make_float2(0.0f, 0.0f);
-    constexpr float kLog2e = 1.4426950408889634f, kGelu = 1.5957691216057308f;  // 2 sqrt(2 / pi)
-    float2 z;  // -z log2(e)
-    if constexpr (GELU) {
-        const float2 a = make_float2(-kGelu * kLog2e, -kGelu * kLog2e), b = make_float2(-kGelu * kLog2e * 0.044715f, -kGelu * kLog2e * 0.044715f);
-        z = fma_f32x2(fma_f32x2(fma_f32x2(t, t, zero), b, a), t, zero);
-    } else {
-        z = fma_f32x2(t, make_float2(-kLog2e, -kLog2e), zero);
-    }
-    const float2 d = add_f32x2(make_float2(exp2_fast(z.x), exp2_fast(z.y)), make_float2(1.0f, 1.0f));
-    return make_float2(t.x * rcp_fast(d.x), t.y * rcp_fast(d.y));
 }
 
 // What an epilogue warp owns in shared memory.
@@ -406,8 +349,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
 #pragma unroll
                     for (int kk = 0; kk < 4; ++kk) {
-                        const uint32_t id = (kk & 1) * 2;  // which two of the cell's four scales
-                        tc_mma_mxf4(d, ad + kk * 2, bd + kk * 2, C::kIdesc | (id << 4) | (id << 29), sfa + (kk >> 1) * 4,
+                        const uint32_t id = idesc_scale_id((kk & 1) * 2);
+                        tc_mma_mxf4(d, ad + kk * 2, bd + kk * 2, C::kIdesc | id, sfa + (kk >> 1) * 4,
                                     sfb + (kk >> 1) * 4 * C::kBTiles + shift, acc);
                         acc = 1;
                     }
@@ -495,7 +438,7 @@ struct PairCfg {
     static constexpr int kNumBars = 2 * kStages + 4 + 1 + 1 + kEpiWarps;
     static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
     static_assert(kSmemBytes <= 232448, "shared memory");
-    static constexpr uint32_t kIdesc = (1u << 7) | (1u << 10) | ((uint32_t)(kTN >> 3) << 17) | (1u << 23) | ((uint32_t)(2 * kTM >> 4) << 24);
+    static constexpr uint32_t kIdesc = idesc_mxf4(2 * kTM, kTN);
 };
 
 __device__ __forceinline__ void tc_copy_scales_pair(uint32_t taddr, uint64_t desc) {
@@ -642,8 +585,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk) {
-                            const uint32_t id = (kk & 1) * 2;  // which two of the cell's four scales
-                            tc_mma_mxf4_pair(d, ad + kk * 2, bd + kk * 2, C::kIdesc | (id << 4) | (id << 29), sfa + (kk >> 1) * 4,
+                            const uint32_t id = idesc_scale_id((kk & 1) * 2);
+                            tc_mma_mxf4_pair(d, ad + kk * 2, bd + kk * 2, C::kIdesc | id, sfa + (kk >> 1) * 4,
                                              sfb + (kk >> 1) * 8, acc);
                             acc = 1;
                         }
@@ -697,36 +640,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(ptr);
-    });
-    return fn;
-}
-
-static qmm_status map_2d(CUtensorMap *map, CUtensorMapDataType type, const void *base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
-                         uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swz) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return fail(QMM_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-    cuuint64_t dims[2] = {inner, outer};
-    cuuint64_t strides[1] = {row_bytes};
-    cuuint32_t box[2] = {box_inner, box_outer};
-    cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, type, 2, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(QMM_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
-    return QMM_OK;
-}
-
 // Scales as [row tiles][256-byte rows]: a stage's two tiles of a row tile are four consecutive rows.
 static qmm_status map_scales(CUtensorMap *map, const uint8_t *scales, int64_t rows, int64_t k, uint32_t row_tiles_a_box) {
     EncodeTiledFn fn = encode_fn();
@@ -739,19 +652,6 @@ static qmm_status map_scales(CUtensorMap *map, const uint8_t *scales, int64_t ro
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t *>(scales), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fail(QMM_ERR_CUDA, "cuTensorMapEncodeTiled (scales) failed (%d)", (int)r);
-    return QMM_OK;
-}
-
-template <typename K>
-static qmm_status allow_smem(K kernel, int bytes, bool (&configured)[64]) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) dev = 0;
-    if (!configured[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-        if (e != cudaSuccess) return cuda_fail(e, "mxfp4 gemm smem attribute");
-        configured[dev] = true;
-    }
     return QMM_OK;
 }
 
@@ -841,9 +741,11 @@ static qmm_status launch_gemm_pair(const qmm_mx4 &w, const qmm_mx4 &x, const qmm
     return e == cudaSuccess ? QMM_OK : cuda_fail(e, "mxfp4 gemm launch");
 }
 
-// Pairs where their 256 x 256 tiles fill at least half of the SM pairs; below
-// that the 128 x 192 tiles keep more SMs busy.
+// Few tokens or few tiles: the kernel that splits k.  Pairs where their 256 x 256
+// tiles fill at least half of the SM pairs; below that the 128 x 192 tiles keep more
+// SMs busy.
 static qmm_status launch_product(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epilogue &ep, uint16_t *y, cudaStream_t st) {
+    if (mx4_small_fits(w.rows, x.rows)) return launch_mx4_small(w, nullptr, 0, 0, x, ep, y, st);
     const int64_t pair_tiles = ((x.rows + 255) / 256) * ((w.rows + 255) / 256);
     if (pair_tiles * 4 >= sm_count()) return launch_gemm_pair(w, x, ep, y, st);
     return launch_gemm<192>(w, x, ep, y, st);
@@ -874,6 +776,11 @@ uint64_t qmm_mx4_workspace_bytes(int64_t m, int64_t k) {
     return round16(qmm_mx4_code_bytes(m, k)) + qmm_mx4_scale_bytes(m, k);
 }
 
+uint64_t qmm_mx4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    return qmm::mx4::mx4_small_fits(n, m) && qmm::mx4::mx4_small_quantises(n, m, k) ? 0 : qmm_mx4_workspace_bytes(m, k);
+}
+
 qmm_status qmm_mx4_linear(const qmm_mx4_linear_args *p, void *stream) {
     if (!p) return fail(QMM_ERR_INVALID_ARGUMENT, "mxfp4 linear: null arguments");
     const qmm_mx4_linear_args &a = *p;
@@ -902,12 +809,12 @@ qmm_status qmm_mx4_linear(const qmm_mx4_linear_args *p, void *stream) {
     const Span sw[] = {span(a.w.codes, qmm_mx4_code_bytes(a.w.rows, a.w.k)), span(a.w.scales, qmm_mx4_scale_bytes(a.w.rows, a.w.k))};
     Span sx[] = {span(a.x_codes, quantised ? code_bytes : 0), span(a.x_scales, quantised ? scale_bytes : 0)};
     qmm_mx4 x{a.x_codes, a.x_scales, a.m, a.w.k};
-    if (!quantised) {
-        const uint64_t need = qmm_mx4_workspace_bytes(a.m, a.w.k);
+    const uint64_t need = quantised ? 0 : qmm_mx4_linear_workspace_bytes(a.m, a.w.rows, a.w.k);
+    if (!quantised) sx[0] = span(a.x, ((uint64_t)(a.m - 1) * (uint64_t)a.x_row_stride + (uint64_t)a.w.k) * xsize);
+    if (need) {
         if (!a.workspace || a.workspace_bytes < need)
             return fail(QMM_ERR_INVALID_ARGUMENT, "mxfp4 linear: workspace of %llu bytes is smaller than %llu", (unsigned long long)a.workspace_bytes, (unsigned long long)need);
         if (misaligned(a.workspace)) return fail(QMM_ERR_MISALIGNED, "mxfp4 linear: workspace is not 16-byte aligned");
-        sx[0] = span(a.x, ((uint64_t)(a.m - 1) * (uint64_t)a.x_row_stride + (uint64_t)a.w.k) * xsize);
         sx[1] = span(a.workspace, need);
         if (overlap(sx[0], sx[1]) || overlap(sx[1], sw[0]) || overlap(sx[1], sw[1]) ||
             (a.residual && overlap(sx[1], span(a.residual, (uint64_t)a.m * (uint64_t)a.w.rows * 2))))
@@ -922,11 +829,12 @@ qmm_status qmm_mx4_linear(const qmm_mx4_linear_args *p, void *stream) {
     qmm_status s = qmm::check_device();
     if (s != QMM_OK) return s;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!quantised) {
+    const qmm_epilogue ep{a.bias, a.gate, a.residual, a.activation};
+    if (!quantised && !need) return qmm::mx4::launch_mx4_small(a.w, a.x, a.x_elem, a.x_row_stride, x, ep, a.y, st);
+    if (need) {
         s = qmm::launch_mx4_quantize(a.x, a.x_elem, a.m, a.w.k, a.x_row_stride, const_cast<uint8_t *>(x.codes), const_cast<uint8_t *>(x.scales), st);
         if (s != QMM_OK) return s;
     }
-    const qmm_epilogue ep{a.bias, a.gate, a.residual, a.activation};
     return qmm::mx4::launch_product(a.w, x, ep, a.y, st);
 }
 

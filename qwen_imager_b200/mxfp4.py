@@ -190,8 +190,9 @@ class MxLinear:
             y = torch.empty((m, n), dtype=torch.bfloat16, device=device)
         work, nbytes = None, 0
         if x_ptr:
-            nbytes = -(-m * w.codes.shape[1] // 16) * 16 + -(-m // 128) * -(-k // 256) * 1024
-            work = torch.empty((nbytes,), dtype=torch.uint8, device=device)
+            nbytes = _block.load().qmm_mx4_linear_workspace_bytes(m, n, k)
+            if nbytes:
+                work = torch.empty((nbytes,), dtype=torch.uint8, device=device)
         _block.run("qmm_mx4_linear", device, _block.LINEAR.pack(
             w.codes.data_ptr(), w.scales.data_ptr(), n, k, m, x_ptr, stride, x_codes, x_scales,
             0 if bias is None else bias.data_ptr(), 0 if gate is None else gate.data_ptr(),

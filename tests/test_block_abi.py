@@ -94,15 +94,20 @@ def test_sizes_of_mxfp4_buffers():
     assert lib.qmm_mx4_scale_bytes(5, 33) == 2 * 512        # one row tile, one 256-column chunk
     assert lib.qmm_mx4_scale_bytes(129, 257) == 2 * 4 * 512
     assert lib.qmm_mx4_workspace_bytes(3, 33) == 3 * 32 + 2 * 512
+    # few tokens are quantised inside the product; the rest need the whole of x
+    assert lib.qmm_mx4_linear_workspace_bytes(1, 18432, 3072) == lib.qmm_mx4_linear_workspace_bytes(4, 64, 64) == 0
+    assert lib.qmm_mx4_linear_workspace_bytes(4096, 3072, 3072) == lib.qmm_mx4_workspace_bytes(4096, 3072)
+    assert lib.qmm_mx4_linear_workspace_bytes(0, 64, 64) == 0
     assert lib.qmm_mx4_code_bytes(0, 33) == lib.qmm_mx4_scale_bytes(4, 0) == 0
 
 
-A = 1 << 20  # an aligned address that nothing dereferences
+A = 1 << 28  # an aligned address that nothing dereferences
+NEED = 4096 * 32 + 32 * 1024
 
 
 def linear(**kw):
-    v = dict(codes=A, scales=2 * A, n=64, k=64, m=4, x=3 * A, stride=64, x_codes=0, x_scales=0, bias=0, gate=0, residual=0, y=4 * A,
-             work=5 * A, bytes=4 * 32 + 1024, elem=0, act=0)
+    v = dict(codes=A, scales=2 * A, n=4096, k=64, m=4096, x=3 * A, stride=64, x_codes=0, x_scales=0, bias=0, gate=0, residual=0, y=4 * A,
+             work=5 * A, bytes=NEED, elem=0, act=0)
     v.update(kw)
     return _block.load().qmm_mx4_linear(_block.LINEAR.pack(*v.values()), None)
 
@@ -126,7 +131,7 @@ def linear(**kw):
     (dict(x=3 * A + 1), _lib.QMM_ERR_MISALIGNED),
     (dict(work=5 * A + 4), _lib.QMM_ERR_MISALIGNED),
     (dict(work=0), _lib.QMM_ERR_INVALID_ARGUMENT),
-    (dict(bytes=4 * 32 + 1023), _lib.QMM_ERR_INVALID_ARGUMENT),
+    (dict(bytes=NEED - 1), _lib.QMM_ERR_INVALID_ARGUMENT),
     (dict(y=3 * A), _lib.QMM_ERR_INVALID_ARGUMENT),                   # y overlaps x
     (dict(y=5 * A + 16), _lib.QMM_ERR_INVALID_ARGUMENT),              # y overlaps the workspace
     (dict(work=3 * A + 16), _lib.QMM_ERR_INVALID_ARGUMENT),           # the workspace overlaps x
