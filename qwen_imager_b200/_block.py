@@ -7,11 +7,14 @@ is the time of its call.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
+import os
 import struct
 
 import torch
 
 from . import _lib
+from . import build as _build
 from ._lib import QmmError
 
 ELEM_BF16, ELEM_F32, ELEM_F16 = 0, 1, 2
@@ -41,6 +44,7 @@ ROTARY = struct.Struct("8PPqq12qq8if4x")          # qmm_rotary_args
 NORM = struct.Struct("11P10q5iff4x")              # qmm_gated_norm_args
 
 _lib_block = None
+_host_module = None
 
 
 def load() -> ctypes.CDLL:
@@ -67,6 +71,29 @@ def load() -> ctypes.CDLL:
     return _lib_block
 
 
+def host():
+    """The extension with the operators' ordinary calls (csrc/host/block_host.cpp),
+    built first when stale: a small operator's time is the time of its call
+    (B200, one-token linear: 14 us through the checks here and ctypes)."""
+    global _host_module
+    if _host_module is None:
+        lib = load()
+        if _build.host_is_stale():
+            try:
+                _build.build_host()
+            except Exception as exc:  # no compiler, or an error: the built one, if any, still serves
+                if not os.path.exists(_build.HOST):
+                    raise QmmError(_lib.QMM_ERR_CUDA, f"_qmm_host.so is not built and cannot be built: {exc}")
+        spec = importlib.util.spec_from_file_location("_qmm_host", _build.HOST)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "qmm_mx4_linear", "qmm_mx4_linear_workspace_bytes", "qmm_mx4_quantize", "qmm_mx4_dequantize", "qmm_qk_norm_rotary",
+            "qmm_gated_residual_norm")))
+        _host_module = module
+    return _host_module
+
+
 def run(name: str, device: torch.device, *args) -> None:
     """Calls entry point `name` on `device` and its current stream."""
     fn = getattr(_lib_block or load(), name)
@@ -78,6 +105,13 @@ def run(name: str, device: torch.device, *args) -> None:
             status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status)
+
+
+def checked(result):
+    """What a call of the extension made, or its status raised."""
+    if result.__class__ is int:
+        _lib.check(result)
+    return result
 
 
 def bad_argument(message: str) -> QmmError:

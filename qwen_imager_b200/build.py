@@ -4,6 +4,7 @@ The library is compiled for sm_100a only and written to
 qwen_imager_b200/_build/libqmm.so, next to the sources, so that it travels with
 the repository to the machine that runs it.  The CUDA runtime is linked
 statically; the driver API entry point for tensor maps is resolved at run time.
+Beside it, _build/_qmm_host.so: the block operators' ordinary calls in C++ (g++).
 
 Usage: python -m qwen_imager_b200.build [--verbose]
 """
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -21,6 +23,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OUT_DIR = os.path.join(PKG, "_build")
 LIB = os.path.join(OUT_DIR, "libqmm.so")
+HOST_SRC = os.path.join(CSRC, "host", "block_host.cpp")
+HOST = os.path.join(OUT_DIR, "_qmm_host.so")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -46,11 +50,42 @@ def headers() -> list[str]:
             + sorted(glob.glob(os.path.join(ROOT, "include", "*.h"))))
 
 
-def is_stale() -> bool:
-    if not os.path.exists(LIB):
+def _older(target: str, files: list[str]) -> bool:
+    if not os.path.exists(target):
         return True
-    built = os.path.getmtime(LIB)
-    return any(os.path.getmtime(f) > built for f in sources() + headers() + [__file__])
+    built = os.path.getmtime(target)
+    return any(os.path.getmtime(f) > built for f in files)
+
+
+def is_stale() -> bool:
+    return _older(LIB, sources() + headers() + [__file__])
+
+
+def host_is_stale() -> bool:
+    return _older(HOST, [HOST_SRC, os.path.join(ROOT, "include", "qmm_block.h"), os.path.join(ROOT, "include", "qmm.h"), __file__])
+
+
+def build_host(force: bool = False) -> str:
+    """Compiles the Python extension of the block operators' calls (g++, against
+    torch's headers; the entry points it calls are bound at run time)."""
+    if not force and not host_is_stale():
+        return HOST
+    import torch
+
+    os.makedirs(OUT_DIR, exist_ok=True)
+    base = os.path.dirname(torch.__file__)
+    inc = os.path.join(base, "include")
+    cuda = os.path.dirname(os.path.dirname(nvcc_path()))
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-I" + os.path.join(ROOT, "include"), "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], HOST_SRC, "-o", HOST + ".tmp",
+           "-L" + os.path.join(base, "lib"), "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("g++ failed on block_host.cpp")
+    os.replace(HOST + ".tmp", HOST)
+    return HOST
 
 
 def build(verbose: bool = False, force: bool = False) -> str:
@@ -90,3 +125,4 @@ def build(verbose: bool = False, force: bool = False) -> str:
 
 if __name__ == "__main__":
     print(build(verbose="--verbose" in sys.argv, force=True))
+    print(build_host(force=True))

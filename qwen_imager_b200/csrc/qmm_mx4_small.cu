@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         pdl_dependency_wait();
         if (quantise) {
             // -------------------------------------------------------- x to MXFP4
-            // unit = (stage, row); a warp's units are kWorkers apart, two in flight
+            // unit = (stage, row); a warp's units are kWorkers apart
             const T *const x = static_cast<const T *>(p.x) + (int64_t)m0 * p.x_row_stride;
             const int units = nkb * tokens;
             auto fetch = [&](int u, float (&v)[8]) {
@@ -260,14 +260,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) mbar_arrive(&xfull[s]);
                 return true;
             };
-            float a[8], b[8];
-            int u = warp;
-            if (u < units) fetch(u, a);
-            for (; ok && u < units; u += 2 * kWorkers) {
-                if (u + kWorkers < units) fetch(u + kWorkers, b);
-                ok = __all_sync(0xffffffffu, put(u, a));
-                if (ok && u + 2 * kWorkers < units) fetch(u + 2 * kWorkers, a);
-                if (ok && u + kWorkers < units) ok = __all_sync(0xffffffffu, put(u + kWorkers, b));
+            constexpr int kFlight = 8;  // units whose loads a warp has in flight
+            for (int u0 = warp; ok && u0 < units; u0 += kFlight * kWorkers) {
+                float v[kFlight][8];
+#pragma unroll
+                for (int j = 0; j < kFlight; ++j)
+                    if (u0 + j * kWorkers < units) fetch(u0 + j * kWorkers, v[j]);
+#pragma unroll
+                for (int j = 0; j < kFlight; ++j)
+                    if (ok && u0 + j * kWorkers < units) ok = __all_sync(0xffffffffu, put(u0 + j * kWorkers, v[j]));
             }
         }
         // ------------------------------------------------------------ epilogue

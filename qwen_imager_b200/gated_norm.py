@@ -33,6 +33,14 @@ def gated_residual_norm(x: torch.Tensor, branch: Optional[torch.Tensor] = None, 
     a batch.  f32 inside, one rounding per output, n from the unrounded x'.
     x_out may be x or branch, n_out may be either too; quantize=True gives n as
     an MxTensor."""
+    if x_out is None and n_out is None:
+        made = _block.host().gated_norm(x, branch, _block.NORMS.get(post, -1), post_weight, gate, residual_scale,
+                                        _block.NORMS.get(pre, -1), pre_weight, scale, shift, eps, quantize)
+        if made is not None:
+            made = _block.checked(made)
+            if not quantize:
+                return made
+            return made[0], MxTensor(made[1], made[2], made[1].shape[0], x.shape[-1], x.shape[:-1])
     device = _block.require_cuda(x, "x")
     x_elem = _block.elem_of(x, "x")
     post_kind, pre_kind = _block.NORMS.get(post), _block.NORMS.get(pre)

@@ -22,6 +22,9 @@ from . import _lib
 
 BLOCK = 32
 
+_host = _block.host
+_checked = _block.checked
+
 
 class MxTensor:
     """An MXFP4 matrix [rows, k] (qmm_mx4 of include/qmm_block.h).
@@ -81,6 +84,10 @@ class MxTensor:
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values, [..., k]; exact in bf16 and f32."""
+        if dtype is torch.bfloat16 and len(self.lead) == 1:
+            out = _host().mx_dequantize(self.codes, self.scales, self.rows, self.k)
+            if out is not None:
+                return _checked(out)
         e = _block.ELEMS.get(dtype)
         if e is None:
             raise bad_argument(f"dequantize does not support {dtype}")
@@ -97,6 +104,11 @@ def mx_quantize(x: torch.Tensor) -> MxTensor:
     Each block's scale is the power of two that brings its largest magnitude
     to [4, 8); values round to the nearest code, ties to the even one, and
     saturate at 6 scales.  A block with an infinity or NaN becomes NaN."""
+    made = _host().mx_quantize(x)
+    if made is not None:
+        codes, scales = _checked(made)
+        lead = x.shape[:-1]
+        return MxTensor(codes, scales, codes.shape[0], x.shape[-1], lead)
     device = _block.require_cuda(x, "input")
     e = _block.elem_of(x, "input")
     if x.dim() == 0 or x.shape[-1] == 0:
@@ -149,7 +161,19 @@ class MxLinear:
         act = ACTIVATIONS.get(activation)
         if act is None:
             raise bad_argument(f"unknown activation {activation!r}")
+        if residual_mul:
+            act |= _lib.QMM_EPILOGUE_RESIDUAL_MUL
         w = self.weight
+        if out is None:
+            b = self.bias if bias is OWN_BIAS else bias
+            if x.__class__ is not MxTensor:
+                y = _host().mx_linear(x, None, w.codes, w.scales, self.output, self.input, b, gate, residual, act)
+            elif x.k == self.input and len(x.lead) == 1:
+                y = _host().mx_linear(x.codes, x.scales, w.codes, w.scales, self.output, self.input, b, gate, residual, act)
+            else:
+                y = None
+            if y is not None:
+                return _checked(y)
         device, n, k = w.codes.device, self.output, self.input
         x_ptr = stride = x_codes = x_scales = elem = 0
         if isinstance(x, MxTensor):
@@ -196,8 +220,7 @@ class MxLinear:
         _block.run("qmm_mx4_linear", device, _block.LINEAR.pack(
             w.codes.data_ptr(), w.scales.data_ptr(), n, k, m, x_ptr, stride, x_codes, x_scales,
             0 if bias is None else bias.data_ptr(), 0 if gate is None else gate.data_ptr(),
-            0 if residual is None else residual.data_ptr(), y.data_ptr(), 0 if work is None else work.data_ptr(), nbytes, elem,
-            act | _lib.QMM_EPILOGUE_RESIDUAL_MUL if residual_mul else act))
+            0 if residual is None else residual.data_ptr(), y.data_ptr(), 0 if work is None else work.data_ptr(), nbytes, elem, act))
         if result is not y:
             result.view(m, n).copy_(y)
         return result

@@ -58,6 +58,7 @@ class RotaryAxes:
         if any(not math.isfinite(f) for f in freq):
             raise bad_argument("a frequency is not finite")
         self.pairs, self.count, self.axes = pairs, len(axis), axes
+        self._adjacent = int(pairs == "adjacent")
         turns = torch.tensor(freq, dtype=torch.float64) / (2.0 * math.pi)
         lead = turns.float()
         self._turns = torch.stack([lead, (turns - lead.double()).float()], -1).contiguous().to(device)
@@ -76,6 +77,11 @@ def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.
     may differ, or None.  positions [tokens, axes], or [batch, tokens, axes]:
     int32, int64 or f32 (whole numbers to 2^24 and fractions exactly).
     Outputs are new contiguous tensors, or q_out / k_out, which may be q / k."""
+    if q_out is None and k_out is None:
+        made = _block.host().qk_norm_rotary(q, k, positions, axes._turns, axes._axis, axes.axes, axes._adjacent, q_weight, k_weight, eps)
+        if made is not None:
+            made = _block.checked(made)
+            return made if k is not None else (made, None)
     device = _block.require_cuda(q, "q")
     elem = _block.elem_of(q, "q")
     batched = q.dim() == 4
@@ -110,7 +116,7 @@ def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.
         q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(), 0 if k is None else k_out.data_ptr(),
         0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(), positions.data_ptr(),
         axes._turns.data_ptr(), axes._axis.data_ptr(), batch, tokens, *qs, *ks, *qo, *ko, pos_stride, q_heads, k_heads, dim,
-        axes.count, axes.axes, axes.pairs == "adjacent", kind, elem, eps))
+        axes.count, axes.axes, axes._adjacent, kind, elem, eps))
     return q_out, (k_out if k is not None else None)
 
 
