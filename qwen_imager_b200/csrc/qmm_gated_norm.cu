@@ -151,6 +151,7 @@ __global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_
     };
     const int64_t pitch = mx4_pitch(hidden), tiles = mx4_scale_tiles(hidden);
 
+    pdl_launch_dependents();  // a product behind this pass sets itself up meanwhile; it waits for the grid before it reads
     fetch(blockIdx.x);
     for (uint32_t row = blockIdx.x; row < (uint32_t)a.rows; row += gridDim.x) {
         const uint32_t group = row / rows_per_group;

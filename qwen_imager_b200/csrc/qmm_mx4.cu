@@ -31,6 +31,7 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantArgs a
     const int64_t row0 = (int64_t)(blockIdx.y >> 2) * 128 + i;
     const int64_t col0 = (int64_t)blockIdx.x * 256;
     const T *x = static_cast<const T *>(a.x);
+    pdl_launch_dependents();  // a product behind this pass sets itself up meanwhile; it waits for the grid before it reads
     if (row0 >= a.rows) return;
     float v[kRows][8];
     if constexpr (VEC) {  // k is a multiple of 8: a lane's columns are all in or all out

@@ -705,9 +705,19 @@ static qmm_status launch_gemm(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epil
     s = make_problem(q, w, x, ep, y, kTM, TN, TN);
     if (s != QMM_OK) return s;
     const unsigned grid = (unsigned)std::min<int64_t>((int64_t)q.p.m_tiles * q.p.n_tiles, sm_count());
-    mx4_gemm_kernel<TN><<<grid, kThreads, C::kSmemBytes, st>>>(q.a, q.b, q.y, q.res, q.p);
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(grid, 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, mx4_gemm_kernel<TN>, q.a, q.b, q.y, q.res, q.p);
     count_launch();
-    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? QMM_OK : cuda_fail(e, "mxfp4 gemm launch");
 }
 
@@ -724,7 +734,7 @@ static qmm_status launch_gemm_pair(const qmm_mx4 &w, const qmm_mx4 &x, const qmm
     if ((s = map_scales(&sfb, w.scales, w.rows, w.k, 2)) != QMM_OK) return s;
     const unsigned pairs = (unsigned)std::min<int64_t>((int64_t)q.p.m_tiles * q.p.n_tiles, std::max(1, sm_count() / 2));
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3(pairs * 2, 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmemBytes;
@@ -733,8 +743,10 @@ static qmm_status launch_gemm_pair(const qmm_mx4 &w, const qmm_mx4 &x, const qmm
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     cudaError_t e = cudaLaunchKernelEx(&cfg, mx4_gemm_pair_kernel, q.a, q.b, sfa, sfb, q.y, q.res, q.p);
     count_launch();
     if (e == cudaSuccess) e = cudaGetLastError();

@@ -7,11 +7,12 @@
 // splits k and sums its partial tiles over distributed shared memory, always in the
 // same order.
 //
-// x needs no pass of its own: eight warps quantise this CTA's columns of it while the
+// x needs no pass of its own: 16 warps quantise this CTA's columns of it while the
 // weight is on its way (a warp a row of 256 columns: eight columns a lane, four lanes a
 // block), writing codes and scales straight into the stage's operand layout; an x that
 // is MXFP4 already comes by TMA instead.  The same warps then run the epilogue.
 #include <algorithm>
+#include <cstring>
 
 #include "qmm_mx4_mma.cuh"
 
@@ -20,7 +21,7 @@ namespace mx4 {
 namespace small {
 
 constexpr int kRows = 128;  // features a tile
-constexpr int kWorkers = 8;
+constexpr int kWorkers = 16;
 constexpr int kProducer = kWorkers, kMma = kWorkers + 1;
 constexpr int kThreads = (kWorkers + 2) * 32;
 constexpr int kMaxSplit = 8;
@@ -60,9 +61,9 @@ struct Params {
     uint32_t *err;
 };
 
-__device__ __forceinline__ float load_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 load_cluster_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
 
@@ -230,69 +231,83 @@ __global__ void __launch_bounds__(kThreads, 1)
             // unit = (stage, row); a warp's units are kWorkers apart
             const T *const x = static_cast<const T *>(p.x) + (int64_t)m0 * p.x_row_stride;
             const int units = nkb * tokens;
-            auto fetch = [&](int u, float (&v)[8]) {
+            constexpr int kFlight = sizeof(T) == 4 ? 4 : 8;  // units whose loads a warp has in flight
+            auto fetch = [&](int u) {
                 const int i = u / tokens, r = u - i * tokens;
                 const int64_t c = (int64_t)(kb0 + i) * kBK + lane * 8;
                 const T *const src = x + (int64_t)r * p.x_row_stride + c;
+                Vec8<T> raw{};
                 if (p.vec) {
-                    Vec8<T> raw{};
                     if (c < p.k) raw = load_vec8(src);
-                    vec8_to_f32(raw, v);
                 } else {
+                    T e[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = c + e < p.k ? elem_to_f32(src[e]) : 0.0f;
+                    for (int j = 0; j < 8; ++j) {
+                        e[j] = T{};
+                        if (c + j < p.k) e[j] = src[j];
+                    }
+                    memcpy(&raw, e, sizeof raw);
                 }
+                return raw;
             };
-            auto put = [&](int u, float (&v)[8]) {
-                const int i = u / tokens, r = u - i * tokens, s = i % S;
-                if (i >= S && !mbar_wait(&empty[s], ((i / S) & 1) ^ 1, p.err, kErrTimeoutDequant)) return false;
-                uint32_t codes;
-                const uint32_t e = mx4_encode8(v, &codes);
-                uint32_t word = e << (8 * ((lane >> 2) & 3));
-                word |= __shfl_xor_sync(0xffffffffu, word, 4);
-                word |= __shfl_xor_sync(0xffffffffu, word, 8);
-                // 16-byte cells of a 128-byte row are swizzled by the row's place in eight
-                *reinterpret_cast<uint32_t *>(smem + C::kBOff + s * C::kBBytes + r * kRowBytes + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = codes;
-                if ((lane & 15) == 0)
-                    *reinterpret_cast<uint32_t *>(smem + C::kSfbOff + s * C::kSfBytes + (lane >> 4) * kSfTile + (r & 31) * 16 + (r >> 5) * 4) = word;
+            // Rows written but not yet announced are units first .. last - 1 (in steps of kWorkers).
+            auto announce = [&](int first, int last) {
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&xfull[s]);
-                return true;
+                if (lane == 0)
+                    for (int u = first; u < last; u += kWorkers) mbar_arrive(&xfull[u / tokens % S]);
             };
-            constexpr int kFlight = 8;  // units whose loads a warp has in flight
             for (int u0 = warp; ok && u0 < units; u0 += kFlight * kWorkers) {
-                float v[kFlight][8];
+                Vec8<T> raw[kFlight];
 #pragma unroll
                 for (int j = 0; j < kFlight; ++j)
-                    if (u0 + j * kWorkers < units) fetch(u0 + j * kWorkers, v[j]);
+                    if (u0 + j * kWorkers < units) raw[j] = fetch(u0 + j * kWorkers);
+                int first = u0;
 #pragma unroll
-                for (int j = 0; j < kFlight; ++j)
-                    if (ok && u0 + j * kWorkers < units) ok = __all_sync(0xffffffffu, put(u0 + j * kWorkers, v[j]));
+                for (int j = 0; j < kFlight; ++j) {
+                    const int u = u0 + j * kWorkers;
+                    if (!ok || u >= units) break;
+                    const int i = u / tokens, r = u - i * tokens, s = i % S;
+                    if (i >= S) {  // the ring's stage is in use: what it waits for may need the rows above
+                        announce(first, u);
+                        first = u;
+                        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((i / S) & 1) ^ 1, p.err, kErrTimeoutDequant));
+                        if (!ok) break;
+                    }
+                    float v[8];
+                    vec8_to_f32(raw[j], v);
+                    uint32_t codes;
+                    const uint32_t e = mx4_encode8(v, &codes);
+                    uint32_t word = e << (8 * ((lane >> 2) & 3));
+                    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+                    word |= __shfl_xor_sync(0xffffffffu, word, 8);
+                    // 16-byte cells of a 128-byte row are swizzled by the row's place in eight
+                    *reinterpret_cast<uint32_t *>(smem + C::kBOff + s * C::kBBytes + r * kRowBytes + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = codes;
+                    if ((lane & 15) == 0)
+                        *reinterpret_cast<uint32_t *>(smem + C::kSfbOff + s * C::kSfBytes + (lane >> 4) * kSfTile + (r & 31) * 16 + (r >> 5) * 4) = word;
+                }
+                if (ok) announce(first, min(u0 + kFlight * kWorkers, units));
             }
         }
         // ------------------------------------------------------------ epilogue
-        const int quad = warp & 3, half = warp >> 2;
+        const int quad = warp & 3, group = warp >> 2;
         const int64_t f = n0 + quad * 32 + lane;
         const FeatureConsts fc = load_feature_consts(p.ep, f, f < p.n);
         ok = ok && __all_sync(0xffffffffu, mbar_wait(acc_full, 0, p.err, kErrTimeoutEpilogue));
         if (ok) {
             tc_fence_after_sync();
-            constexpr int kCols = NT / 2 < 32 ? NT / 2 : 32;
+            constexpr int kCols = NT / 4 < 8 ? 8 : NT / 4;  // tokens a warp (16: two of the four groups)
             float *const part = reinterpret_cast<float *>(smem + C::kAOff);  // [NT][kRows]: every MMA on the ring is complete
+            const int t0 = group * kCols;
+            if (t0 < tokens) {
+                uint32_t r[kCols];
+                tmem_ld(tmem + ((uint32_t)(quad * 32) << 16) + t0, r);
+                tc_wait_ld();
 #pragma unroll
-            for (int c0 = 0; c0 < NT / 2; c0 += kCols) {
-                const int t0 = half * (NT / 2) + c0;
-                if (t0 < tokens) {
-                    uint32_t r[kCols];
-                    tmem_ld(tmem + ((uint32_t)(quad * 32) << 16) + t0, r);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int c = 0; c < kCols; ++c) {
-                        if (t0 + c < tokens) {
-                            if (split > 1) part[(t0 + c) * kRows + quad * 32 + lane] = __uint_as_float(r[c]);
-                            else if (f < p.n) finish(p, __uint_as_float(r[c]), fc.bias, fc.gate, m0 + t0 + c, f);
-                        }
+                for (int c = 0; c < kCols; ++c) {
+                    if (t0 + c < tokens) {
+                        if (split > 1) part[(t0 + c) * kRows + quad * 32 + lane] = __uint_as_float(r[c]);
+                        else if (f < p.n) finish(p, __uint_as_float(r[c]), fc.bias, fc.gate, m0 + t0 + c, f);
                     }
                 }
             }
@@ -306,19 +321,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         // anywhere the sums are of no use, as the error word says.)
         __syncthreads();
         cluster_sync();
-        if (warp < kWorkers) {
-            const int col = threadIdx.x & (kRows - 1);
-            const int64_t f = n0 + col;
-            const FeatureConsts fc = load_feature_consts(p.ep, f, f < p.n);
-            const uint32_t part = smem_u32(smem + C::kAOff) + col * 4;
-            for (int t = rank + split * (threadIdx.x / kRows); t < tokens; t += split * (kWorkers * 32 / kRows)) {
-                float v[kMaxSplit];
+        if (warp < kWorkers) {  // a warp a token, four features a lane
+            const int64_t f = n0 + lane * 4;
+            FeatureConsts fc[4];
 #pragma unroll
-                for (int j = 0; j < kMaxSplit; ++j) v[j] = j < split ? load_cluster_f32(mapa_shared(part + t * kRows * 4, j)) : 0.0f;
-                float s = v[0];
+            for (int i = 0; i < 4; ++i) fc[i] = load_feature_consts(p.ep, f + i, f + i < p.n);
+            const uint32_t part = smem_u32(smem + C::kAOff) + lane * 16;
+            for (int t = rank + split * warp; t < tokens; t += split * kWorkers) {
+                float4 v[kMaxSplit];
 #pragma unroll
-                for (int j = 1; j < kMaxSplit; ++j) s += v[j];
-                if (f < p.n) finish(p, s, fc.bias, fc.gate, m0 + t, f);
+                for (int j = 0; j < kMaxSplit; ++j) v[j] = j < split ? load_cluster_f32x4(mapa_shared(part + t * kRows * 4, j)) : float4{};
+                float4 s = v[0];
+#pragma unroll
+                for (int j = 1; j < kMaxSplit; ++j) s.x += v[j].x, s.y += v[j].y, s.z += v[j].z, s.w += v[j].w;
+                if (f < p.n) finish(p, s.x, fc[0].bias, fc[0].gate, m0 + t, f);
+                if (f + 1 < p.n) finish(p, s.y, fc[1].bias, fc[1].gate, m0 + t, f + 1);
+                if (f + 2 < p.n) finish(p, s.z, fc[2].bias, fc[2].gate, m0 + t, f + 2);
+                if (f + 3 < p.n) finish(p, s.w, fc[3].bias, fc[3].gate, m0 + t, f + 3);
             }
         }
         cluster_sync();  // no CTA leaves while another reads its partial tile
@@ -378,12 +397,14 @@ static qmm_status launch(const qmm_mx4 &w, const void *x, int64_t x_row_stride, 
     return e == cudaSuccess ? QMM_OK : cuda_fail(e, "mxfp4 product launch");
 }
 
-// CTAs along k: as many as keep the grid within `sms`, so that few tiles still read
-// the weight with most of the machine.
+// CTAs along k: as many as keep the grid within `sms`, where that takes eight stages
+// or more out of a CTA's way: a stage costs 0.24 us, the cluster's sum about 1.2 us
+// (B200, one token: 12288 -> 3072 7.6 us split against 15.3, 3072 -> 3072 4.8 against
+// 5.2; 3072 -> 9216 in two 6.2 against 5.8).
 static int split_for(int64_t tiles, int64_t nkb, int sms) {
     int split = 1;
     while (split < kMaxSplit && split * 2 <= nkb && tiles * split * 2 <= sms) split *= 2;
-    return split;
+    return nkb - (nkb + split - 1) / split >= 8 ? split : 1;
 }
 
 // Tokens a tile for m tokens, and the tiles.
@@ -407,12 +428,12 @@ bool mx4_small_fits(int64_t n, int64_t m) {
 }
 
 bool mx4_small_quantises(int64_t n, int64_t m, int64_t k) {
-    // Every tile of features quantises its columns of x for itself.  Up to 32
-    // vectors of columns a thread that hides behind the weight's arrival; past it a
-    // pass of its own over x is shorter.
+    // Every tile of features quantises its columns of x for itself.  Up to two rows
+    // of a stage a warp that costs less than a pass of its own over x (B200, 4 x 3072
+    // -> 9216: 7.6 us against 8.2; 37 x 1152 -> 3456, five a warp: 8.9 against 7.9).
     const qmm_mx4 w{nullptr, nullptr, n, k};
     const int64_t nkb = (k + kBK - 1) / kBK, split = small::split_for(small::tiles_for(w, m), nkb, kSms);
-    return (nkb + split - 1) / split * std::min<int64_t>(m, small::tile_for(m)) <= 32 * small::kWorkers;
+    return (nkb + split - 1) / split * std::min<int64_t>(m, small::tile_for(m)) <= 2 * small::kWorkers;
 }
 
 qmm_status launch_mx4_small(const qmm_mx4 &w, const void *x, int32_t elem, int64_t x_row_stride, const qmm_mx4 &xq, const qmm_epilogue &ep,
