@@ -3,15 +3,20 @@
 //   x' = residual_scale * x + gate * h
 //   n  = norm_pre(x') * pre_weight * (1 + scale) + shift
 // HBM-bound: x and branch are read once, x' and n (or its MXFP4 codes) written
-// once; the weights and modulation stay in L1.  A CTA takes a row at a time and
-// keeps it in registers (eight columns a vector, up to four vectors a thread), so
-// mean and variance are two passes over registers, and each statistic costs one
-// shuffle tree, one shared slot a warp and one barrier.  The grid is what is
-// resident at once; each CTA loads its next row while it works on this one.
+// once.  A CTA takes a row at a time and keeps it in registers (eight columns a
+// vector, up to four vectors a thread), so mean and variance are two passes over
+// registers, and each statistic costs one shuffle tree, one shared slot a warp and one
+// barrier.  The grid is what is resident at once, consecutive rows to a CTA; it loads
+// its next row while it works on this one.  Weights and modulation enter a row as three vectors, A =
+// post_weight * gate, S = pre_weight * (1 + scale) and H = shift, formed once a CTA
+// (and group) in shared memory, and arithmetic goes two columns an instruction:
+// with the vectors loaded and converted row by row the kernel was bound by its
+// instructions (16896 x 3072 bf16: 116 us).
 // Rows that are not 16-byte aligned take a kernel with columns dealt out one by
 // one (thread t holds columns t, t + T, ...), which keeps accesses of a warp
-// consecutive.
+// consecutive; so do rows past 16384 columns, whose vectors do not fit.
 #include <algorithm>
+#include <type_traits>
 
 #include "qmm_internal.h"
 #include "qmm_mx4.cuh"
@@ -49,39 +54,44 @@ __device__ __forceinline__ void raw8_to_f32(const Raw8<BYTES> &r, bool f16, floa
         vec8_to_f32(t, v);
     }
 }
-__device__ __forceinline__ void load8(const void *p, int elem, int64_t index, float (&v)[8]) {
-    if (elem == QMM_ELEM_F32) raw8_to_f32(load_raw8<4>(p, index), false, v);
-    else raw8_to_f32(load_raw8<2>(p, index), elem == QMM_ELEM_F16, v);
-}
 __device__ __forceinline__ float load_elem(const void *p, int elem, int64_t i) {
     if (elem == QMM_ELEM_F32) return static_cast<const float *>(p)[i];
     if (elem == QMM_ELEM_F16) return elem_to_f32(static_cast<const F16 *>(p)[i]);
     return elem_to_f32(static_cast<const Bf16 *>(p)[i]);
 }
 
-// Sums over a row: a CTA holds it in VPT x 8 columns a thread.  Four slots taken in
-// turn: a slot is written again three barriers after its readers passed theirs.
+// Sums over a row, spread over the CTA's warps (SLOTS at most, a multiple of four).
+// Four sets of slots taken in turn: a set is written again three barriers after its
+// readers passed theirs.  The slots of warps that are not there stay 0.
+template <int SLOTS>
 struct RowSum {
-    float (&red)[4][32];
-    int slot = 0;
+    float (&red)[4][SLOTS];
+    int set = 0;
+    __device__ __forceinline__ RowSum(float (&r)[4][SLOTS]) : red(r) {
+        for (int i = threadIdx.x; i < 4 * SLOTS; i += blockDim.x) (&red[0][0])[i] = 0.0f;
+        __syncthreads();
+    }
     __device__ __forceinline__ float operator()(float s) {
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (warps > 1) {
-            if (lane == 0) red[slot][warp] = s;
+        if (blockDim.x > 32) {
+            if ((threadIdx.x & 31) == 0) red[set][threadIdx.x >> 5] = s;
             __syncthreads();
             s = 0.0f;
-            for (int w = 0; w < warps; ++w) s += red[slot][w];  // the same order in every thread
-            slot = (slot + 1) & 3;
+#pragma unroll
+            for (int w = 0; w < SLOTS; w += 4) {  // the same order in every thread
+                const float4 v = *reinterpret_cast<const float4 *>(&red[set][w]);
+                s += (v.x + v.y) + (v.z + v.w);
+            }
+            set = (set + 1) & 3;
         }
         return s;
     }
 };
 
 // v = norm(v); columns past the row (valid(i, q) false) are 0 and stay 0.
-template <int VPT, typename Valid>
-__device__ __forceinline__ void normalise(float (&v)[VPT][8], int kind, float inv_hidden, float eps, RowSum &row_sum, const Valid &valid) {
+template <int VPT, typename Sum, typename Valid>
+__device__ __forceinline__ void normalise(float (&v)[VPT][8], int kind, float inv_hidden, float eps, Sum &row_sum, const Valid &valid) {
     if (kind == QMM_NORM_LAYER) {
         float s = 0.0f;
 #pragma unroll
@@ -106,18 +116,20 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][8], int kind, float in
         for (int q = 0; q < 8; ++q) v[i][q] *= r;
 }
 
-// Every row of every operand 16-byte aligned, hidden a multiple of 8.
+// x and branch rows, and outputs, 16-byte aligned; hidden a multiple of 8.
 template <typename T, int BBYTES, int VPT, int MAXT, int MINB>
-__global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group) {
-    __shared__ float red[4][32];
-    RowSum row_sum{red};
+__global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group, const uint32_t rows_per_cta,
+                                                                  const bool vec_aligned) {
+    extern __shared__ float4 vectors[];  // A, S, H: threads * VPT * 8 columns each (0 past the row), every thread's its own
+    __shared__ __align__(16) float red[4][MAXT / 32];
+    RowSum<MAXT / 32> row_sum{red};
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
     const int hidden = (int)a.hidden;
     const float inv_hidden = 1.0f / (float)hidden;
     auto column = [&](int i) { return (i * threads + tid) * 8; };
-    auto valid = [&](int i, int) { return column(i) < hidden; };
     constexpr int XB = (int)sizeof(T);
-    const bool xf16 = a.x_elem == QMM_ELEM_F16, bf16_branch = a.branch_elem != QMM_ELEM_F16;
+    const bool f16_branch = a.branch_elem == QMM_ELEM_F16;
+    const int span = threads * VPT * 2;  // float4 a vector
 
     Raw8<XB> rx[VPT];
     Raw8<BBYTES> rb[VPT];
@@ -132,65 +144,153 @@ __global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_
             }
         }
     };
-    auto store = [&](void *p, int64_t base, const float (&v)[VPT][8]) {
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-            if (column(i) < hidden) store_vec8(static_cast<T *>(p) + base + column(i), v[i]);
-    };
-    // v[i][q] = f(v[i][q], vec[base + column])
-    auto with = [&](const void *vec, int64_t base, float (&v)[VPT][8], auto f) {
+    auto store = [&](void *p, int64_t base, const float2 (&v)[VPT][4]) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             if (column(i) < hidden) {
-                float w[8];
-                load8(vec, a.vec_elem, base + column(i), w);
-#pragma unroll
-                for (int q = 0; q < 8; ++q) v[i][q] = f(v[i][q], w[q]);
+                const float w[8] = {v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y, v[i][2].x, v[i][2].y, v[i][3].x, v[i][3].y};
+                store_vec8(static_cast<T *>(p) + base + column(i), w);
             }
         }
+    };
+    // This thread's eight columns of vector `which`.
+    auto mine = [&](int which, int i) { return vectors + which * span + (i * threads + tid) * 2; };
+    auto vec8 = [&](int which, int i, float2 (&w)[4]) {
+        const float4 *q = mine(which, i);
+        const float4 lo = q[0], hi = q[1];
+        w[0] = make_float2(lo.x, lo.y), w[1] = make_float2(lo.z, lo.w), w[2] = make_float2(hi.x, hi.y), w[3] = make_float2(hi.z, hi.w);
+    };
+    // Forms this thread's columns of A, S and H; every load is on its way before the first is used.
+    auto take_vectors = [&](uint32_t group) {
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = column(i);
+            const bool in = c < hidden;
+            const void *const src[5] = {a.post_weight, a.gate, a.pre_weight, a.scale, a.shift};
+            const int64_t at[5] = {c, group * a.gate_stride + c, c, group * a.scale_stride + c, group * a.shift_stride + c};
+            Raw8<4> raw[5];
+            float w[5][8];
+            const float one = in ? 1.0f : 0.0f;
+            if (vec_aligned) {
+#pragma unroll
+                for (int k = 0; k < 5; ++k) {
+                    raw[k] = Raw8<4>{};
+                    if (in && src[k]) {
+                        if (a.vec_elem == QMM_ELEM_F32) raw[k] = load_raw8<4>(src[k], at[k]);
+                        else raw[k].w[0] = load_raw8<2>(src[k], at[k]).w[0];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 5; ++k) {
+                    if (a.vec_elem == QMM_ELEM_F32) raw8_to_f32(raw[k], false, w[k]);
+                    else raw8_to_f32(Raw8<2>{{raw[k].w[0]}}, a.vec_elem == QMM_ELEM_F16, w[k]);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 5; ++k)
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) w[k][q] = in && src[k] ? load_elem(src[k], a.vec_elem, at[k] + q) : 0.0f;
+            }
+            float *const fa = reinterpret_cast<float *>(mine(0, i)), *const fs = reinterpret_cast<float *>(mine(1, i)), *const fh = reinterpret_cast<float *>(mine(2, i));
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const float pw = src[0] ? w[0][q] : one, g = src[1] ? w[1][q] : 1.0f, qw = src[2] ? w[2][q] : one;
+                fa[q] = pw * g;
+                fs[q] = fmaf(qw, w[3][q], qw);
+                fh[q] = w[4][q];
+            }
+        }
+    };
+    // v -= mean, for the sums of squares of a layer norm (columns past the row stay 0).
+    auto centre = [&](float2 (&v)[VPT][4]) {
+        float2 s = twice(0.0f);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s = add_f32x2(s, v[i][q]);
+        const float mean = row_sum(s.x + s.y) * inv_hidden;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const float2 m = twice(column(i) < hidden ? -mean : 0.0f);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[i][q] = add_f32x2(v[i][q], m);
+        }
+    };
+    auto rms = [&](const float2 (&v)[VPT][4]) {
+        float2 s = twice(0.0f);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s = fma_f32x2(v[i][q], v[i][q], s);
+        return rsqrtf(row_sum(s.x + s.y) * inv_hidden + a.eps);
     };
     const int64_t pitch = mx4_pitch(hidden), tiles = mx4_scale_tiles(hidden);
 
     pdl_launch_dependents();  // a product behind this pass sets itself up meanwhile; it waits for the grid before it reads
-    fetch(blockIdx.x);
-    for (uint32_t row = blockIdx.x; row < (uint32_t)a.rows; row += gridDim.x) {
-        const uint32_t group = row / rows_per_group;
-        float x[VPT][8], h[VPT][8];
+    const uint32_t first = blockIdx.x * rows_per_cta, last = min(first + rows_per_cta, (uint32_t)a.rows);
+    fetch(first);
+    uint32_t group = UINT32_MAX;
+    for (uint32_t row = first; row < last; ++row) {
+        if (row / rows_per_group != group) {
+            group = row / rows_per_group;
+            take_vectors(group);
+        }
+        float2 x[VPT][4], h[VPT][4];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            raw8_to_f32(rx[i], xf16, x[i]);
-            raw8_to_f32(rb[i], !bf16_branch, h[i]);
+            float w[8];
+            raw8_to_f32(rx[i], std::is_same<T, F16>::value, w);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[i][q] = make_float2(w[2 * q], w[2 * q + 1]);
+            raw8_to_f32(rb[i], f16_branch, w);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) h[i][q] = make_float2(w[2 * q], w[2 * q + 1]);
         }
-        if (row + gridDim.x < (uint32_t)a.rows) fetch((int64_t)row + gridDim.x);
+        if (row + 1 < last) fetch((int64_t)row + 1);
+        const float2 c2 = twice(a.residual_scale);
         if (a.branch) {
-            if (a.post != QMM_NORM_NONE) normalise(h, a.post, inv_hidden, a.eps, row_sum, valid);
-            if (a.post_weight) with(a.post_weight, 0, h, [](float v, float w) { return v * w; });
-            if (a.gate) with(a.gate, group * a.gate_stride, h, [](float v, float w) { return v * w; });
+            if (a.post == QMM_NORM_LAYER) centre(h);
+            const float2 r = twice(a.post != QMM_NORM_NONE ? rms(h) : 1.0f);
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) {
+                float2 w[4];
+                vec8(0, i, w);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x[i][q] = fma_f32x2(x[i][q], c2, mul_f32x2(mul_f32x2(h[i][q], r), w[q]));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x[i][q] = mul_f32x2(x[i][q], c2);
         }
-#pragma unroll
-        for (int i = 0; i < VPT; ++i)
-#pragma unroll
-            for (int q = 0; q < 8; ++q) x[i][q] = fmaf(a.residual_scale, x[i][q], h[i][q]);
         if (a.x_out) store(a.x_out, row * a.x_out_stride, x);
         if (!a.n_out && !a.n_codes) continue;
-        if (a.pre != QMM_NORM_NONE) normalise(x, a.pre, inv_hidden, a.eps, row_sum, valid);
-        if (a.pre_weight) with(a.pre_weight, 0, x, [](float v, float w) { return v * w; });
-        if (a.scale) with(a.scale, group * a.scale_stride, x, [](float v, float w) { return fmaf(v, w, v); });
-        if (a.shift) with(a.shift, group * a.shift_stride, x, [](float v, float w) { return v + w; });
+        if (a.pre == QMM_NORM_LAYER) centre(x);
+        const float2 r = twice(a.pre != QMM_NORM_NONE ? rms(x) : 1.0f);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            float2 w[4], s[4];
+            vec8(1, i, w);
+            vec8(2, i, s);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[i][q] = fma_f32x2(mul_f32x2(x[i][q], r), w[q], s[q]);
+        }
         if (a.n_out) {
             store(a.n_out, row * a.n_out_stride, x);
             continue;
         }
-        // MXFP4: columns past the row are zeros of its last block.
+        // MXFP4: columns past the row are zeros of its last block (their S and H are 0).
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const int c = column(i);
-            if (c >= hidden) {
+            float w[8] = {x[i][0].x, x[i][0].y, x[i][1].x, x[i][1].y, x[i][2].x, x[i][2].y, x[i][3].x, x[i][3].y};
+            if (c >= hidden) {  // (0 times an infinite or NaN statistic)
 #pragma unroll
-                for (int q = 0; q < 8; ++q) x[i][q] = 0.0f;
+                for (int q = 0; q < 8; ++q) w[q] = 0.0f;
             }
             uint32_t codes;
-            const uint32_t e = mx4_encode8(x[i], &codes);
+            const uint32_t e = mx4_encode8(w, &codes);
             if (c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = codes;
             uint32_t word = e << (8 * ((lane >> 2) & 3));
             word |= __shfl_xor_sync(0xffffffffu, word, 4);
@@ -204,8 +304,8 @@ __global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_
 // Any alignment and width.
 template <typename T, int VPT, int MAXT>
 __global__ void __launch_bounds__(MAXT) gated_norm_any_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group) {
-    __shared__ float red[4][32];
-    RowSum row_sum{red};
+    __shared__ __align__(16) float red[4][MAXT / 32];
+    RowSum<MAXT / 32> row_sum{red};
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
     const int64_t row = blockIdx.x;
     const int hidden = (int)a.hidden;
@@ -291,45 +391,49 @@ static unsigned threads_for(int64_t hidden) {
 }
 
 template <typename T, int BBYTES, int VPT, int MAXT, int MINB>
-static void launch_rows(const qmm_gated_norm_args &a, uint32_t rpg, cudaStream_t st) {
+static cudaError_t launch_rows(const qmm_gated_norm_args &a, uint32_t rpg, bool vec_aligned, cudaStream_t st) {
     auto kernel = gated_norm_kernel<T, BBYTES, VPT, MAXT, MINB>;
     const unsigned threads = threads_for<VPT>(a.hidden);
+    const size_t smem = (size_t)threads * VPT * 8 * 4 * 3;
     static int resident[64][33] = {};  // CTAs an SM by device and warps
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
     int &n = resident[dev][threads / 32];
     if (n == 0) {
         int m = 0;
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&m, kernel, (int)threads, 0) != cudaSuccess || m < 1) m = 1;
-        n = m;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAXT * VPT * 8 * 4 * 3);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&m, kernel, (int)threads, smem);
+        if (e != cudaSuccess) return e;
+        n = std::max(1, m);
     }
-    const unsigned grid = (unsigned)std::min<int64_t>(a.rows, (int64_t)sm_count() * n);
-    kernel<<<grid, threads, 0, st>>>(a, rpg);
+    // Consecutive rows to a CTA: few of them cross into another group's vectors.
+    const int64_t per = (a.rows + (int64_t)sm_count() * n - 1) / ((int64_t)sm_count() * n);
+    kernel<<<(unsigned)((a.rows + per - 1) / per), threads, smem, st>>>(a, rpg, (uint32_t)per, vec_aligned);
+    return cudaGetLastError();
 }
 
 template <typename T, int BBYTES>
-static void launch_fast(const qmm_gated_norm_args &a, uint32_t rpg, cudaStream_t st) {
-    if (a.hidden <= 1024) launch_rows<T, BBYTES, 1, 128, 8>(a, rpg, st);
-    else if (a.hidden <= 4096) launch_rows<T, BBYTES, 2, 256, 3>(a, rpg, st);
-    else if (a.hidden <= 8192) launch_rows<T, BBYTES, 4, 256, 1>(a, rpg, st);
-    else if (a.hidden <= 16384) launch_rows<T, BBYTES, 4, 512, 1>(a, rpg, st);
-    else launch_rows<T, BBYTES, 4, 1024, 1>(a, rpg, st);
+static cudaError_t launch_fast(const qmm_gated_norm_args &a, uint32_t rpg, bool vec_aligned, cudaStream_t st) {
+    if (a.hidden <= 2048) return launch_rows<T, BBYTES, 1, 256, 4>(a, rpg, vec_aligned, st);
+    if (a.hidden <= 4096) return launch_rows<T, BBYTES, 2, 256, 3>(a, rpg, vec_aligned, st);
+    if (a.hidden <= 8192) return launch_rows<T, BBYTES, 4, 256, 1>(a, rpg, vec_aligned, st);
+    return launch_rows<T, BBYTES, 4, 512, 1>(a, rpg, vec_aligned, st);
 }
 
 template <typename T>
-static void launch_any(const qmm_gated_norm_args &a, uint32_t rpg, cudaStream_t st) {
+static cudaError_t launch_any(const qmm_gated_norm_args &a, uint32_t rpg, cudaStream_t st) {
     const unsigned grid = (unsigned)a.rows;
     if (a.hidden <= 1024) gated_norm_any_kernel<T, 1, 128><<<grid, threads_for<1>(a.hidden), 0, st>>>(a, rpg);
     else if (a.hidden <= 4096) gated_norm_any_kernel<T, 2, 256><<<grid, threads_for<2>(a.hidden), 0, st>>>(a, rpg);
     else if (a.hidden <= 16384) gated_norm_any_kernel<T, 4, 512><<<grid, threads_for<4>(a.hidden), 0, st>>>(a, rpg);
     else gated_norm_any_kernel<T, 4, 1024><<<grid, threads_for<4>(a.hidden), 0, st>>>(a, rpg);
+    return cudaGetLastError();
 }
 
 template <typename T>
-static void launch(const qmm_gated_norm_args &a, bool fast, uint32_t rpg, cudaStream_t st) {
-    if (!fast) launch_any<T>(a, rpg, st);
-    else if (a.branch_elem == QMM_ELEM_F32) launch_fast<T, 4>(a, rpg, st);
-    else launch_fast<T, 2>(a, rpg, st);
+static cudaError_t launch(const qmm_gated_norm_args &a, bool fast, bool vec_aligned, uint32_t rpg, cudaStream_t st) {
+    if (!fast) return launch_any<T>(a, rpg, st);
+    return a.branch_elem == QMM_ELEM_F32 ? launch_fast<T, 4>(a, rpg, vec_aligned, st) : launch_fast<T, 2>(a, rpg, vec_aligned, st);
 }
 
 }  // namespace gnorm
@@ -423,16 +527,15 @@ extern "C" qmm_status qmm_gated_residual_norm(const qmm_gated_norm_args *p, void
     auto aligned_vec = [&](const void *q, int64_t stride) {
         return !q || ((reinterpret_cast<uintptr_t>(q) & 15) == 0 && (a.groups == 1 || (stride * vs) % 16 == 0));
     };
-    const bool vec = a.hidden % 8 == 0 && aligned(a.x, a.x_stride, xs) && aligned(a.branch, a.branch_stride, bs) &&
-                     aligned(a.x_out, a.x_out_stride, xs) && aligned(a.n_out, a.n_out_stride, xs) && aligned_vec(a.post_weight, 0) &&
-                     aligned_vec(a.pre_weight, 0) && aligned_vec(a.gate, a.gate_stride) && aligned_vec(a.shift, a.shift_stride) &&
-                     aligned_vec(a.scale, a.scale_stride);
+    const bool vec_aligned = aligned_vec(a.post_weight, 0) && aligned_vec(a.pre_weight, 0) && aligned_vec(a.gate, a.gate_stride) &&
+                             aligned_vec(a.shift, a.shift_stride) && aligned_vec(a.scale, a.scale_stride);
+    const bool vec = a.hidden % 8 == 0 && a.hidden <= 16384 && aligned(a.x, a.x_stride, xs) && aligned(a.branch, a.branch_stride, bs) &&
+                     aligned(a.x_out, a.x_out_stride, xs) && aligned(a.n_out, a.n_out_stride, xs);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint32_t rpg = (uint32_t)(a.rows / a.groups);
-    if (a.x_elem == QMM_ELEM_F32) qmm::gnorm::launch<float>(a, vec, rpg, st);
-    else if (a.x_elem == QMM_ELEM_F16) qmm::gnorm::launch<qmm::F16>(a, vec, rpg, st);
-    else qmm::gnorm::launch<qmm::Bf16>(a, vec, rpg, st);
+    const cudaError_t e = a.x_elem == QMM_ELEM_F32   ? qmm::gnorm::launch<float>(a, vec, vec_aligned, rpg, st)
+                          : a.x_elem == QMM_ELEM_F16 ? qmm::gnorm::launch<qmm::F16>(a, vec, vec_aligned, rpg, st)
+                                                     : qmm::gnorm::launch<qmm::Bf16>(a, vec, vec_aligned, rpg, st);
     qmm::count_launch();
-    const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? QMM_OK : qmm::cuda_fail(e, "gated norm launch");
 }

@@ -90,6 +90,18 @@ __device__ __forceinline__ uint32_t mx4_encode8(float (&v)[8], uint32_t *codes) 
     return e;
 }
 
+__device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
+    uint64_t d;
+    asm("{\n\t.reg .b64 ra, rb;\n\t"
+        "mov.b64 ra, {%1, %2};\n\t"
+        "mov.b64 rb, {%3, %4};\n\t"
+        "mul.rn.f32x2 %0, ra, rb;\n\t}\n"
+        : "=l"(d)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return make_float2(__uint_as_float(static_cast<uint32_t>(d)), __uint_as_float(static_cast<uint32_t>(d >> 32)));
+}
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+
 // ---------------------------------------------------------------- elements
 // Typed loads and stores of the block operators (T: uint16_t tag types below
 // or float).

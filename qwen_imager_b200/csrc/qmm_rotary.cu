@@ -6,7 +6,7 @@
 // four pairs of every head (as two runs of four columns), so the token's sines
 // and cosines are computed once per lane and, multiplied with the norm's weight,
 // stay in registers over the heads; a head of 8 U columns takes U lanes, and
-// 32 / U heads (rounded down) go at a time.
+// 32 / U heads (rounded down) go at a time.  Arithmetic goes two columns an instruction.
 //
 // The angle is positions * turns in turns.  With turns = f + g (leading and
 // trailing term), p = fl(pos f) and e = pos f - p exact by one fma, the fraction
@@ -18,7 +18,7 @@ namespace qmm {
 namespace rotary {
 
 constexpr int kWarps = 4;
-constexpr int kAhead = 4;  // heads in flight per lane group
+constexpr int kResident = 8;  // CTAs an SM: 32 warps cover the loads (B200, 16896 x 48 heads x 128: 72.8 us; with 16 warps 94.9, with 40 78.8)
 
 __device__ __forceinline__ float position_of(const qmm_rotary_args &a, int64_t batch, int64_t token, int axis) {
     const int64_t i = batch * a.pos_batch_stride + token * a.axes + axis;
@@ -36,20 +36,22 @@ __device__ __forceinline__ void pair_turn(const qmm_rotary_args &a, int64_t batc
     sincospif(2.0f * t, s, c);
 }
 
-// Eight elements as two runs of four, each at an address aligned to four
-// elements; ADJ: the runs are neighbours at an address aligned to eight.
+// How a lane's eight columns lie: one run of eight with adjacent pairs, at an address
+// aligned to eight elements; the same aligned to four; two runs of four (halves).
+enum Layout { kWide, kAdjacent, kHalves };
+
 template <typename T>
 struct Runs {
     uint32_t w[sizeof(T) * 2];
 };
-template <typename T, bool ADJ>
+template <typename T, Layout L>
 __device__ __forceinline__ Runs<T> load_runs(const T *p, int ca, int cb) {
     Runs<T> r;
     if constexpr (sizeof(T) == 4) {
         const uint4 a = *reinterpret_cast<const uint4 *>(p + ca), b = *reinterpret_cast<const uint4 *>(p + cb);
         r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
         r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
-    } else if constexpr (ADJ) {
+    } else if constexpr (L == kWide) {
         const uint4 a = *reinterpret_cast<const uint4 *>(p + ca);
         r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
     } else {
@@ -58,8 +60,10 @@ __device__ __forceinline__ Runs<T> load_runs(const T *p, int ca, int cb) {
     }
     return r;
 }
-template <typename T>
-__device__ __forceinline__ void runs_to_f32(const Runs<T> &r, float (&v)[8]) {
+// The first and second members of the lane's four pairs, two pairs a float2.
+template <typename T, Layout L>
+__device__ __forceinline__ void runs_to_pairs(const Runs<T> &r, float2 (&a)[2], float2 (&b)[2]) {
+    float v[8];
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.w[i]);
@@ -71,13 +75,34 @@ __device__ __forceinline__ void runs_to_f32(const Runs<T> &r, float (&v)[8]) {
             v[2 * i + 1] = f.y;
         }
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (L == kHalves) {
+            a[i] = make_float2(v[2 * i], v[2 * i + 1]);
+            b[i] = make_float2(v[4 + 2 * i], v[4 + 2 * i + 1]);
+        } else {
+            a[i] = make_float2(v[4 * i], v[4 * i + 2]);
+            b[i] = make_float2(v[4 * i + 1], v[4 * i + 3]);
+        }
+    }
 }
-template <typename T, bool ADJ>
-__device__ __forceinline__ void store_runs(T *p, int ca, int cb, const float (&v)[8]) {
+template <typename T, Layout L>
+__device__ __forceinline__ void store_pairs(T *p, int ca, int cb, const float2 (&a)[2], const float2 (&b)[2]) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if constexpr (L == kHalves) {
+            v[2 * i] = a[i].x, v[2 * i + 1] = a[i].y;
+            v[4 + 2 * i] = b[i].x, v[4 + 2 * i + 1] = b[i].y;
+        } else {
+            v[4 * i] = a[i].x, v[4 * i + 2] = a[i].y;
+            v[4 * i + 1] = b[i].x, v[4 * i + 3] = b[i].y;
+        }
+    }
     if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<float4 *>(p + ca) = make_float4(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<float4 *>(p + cb) = make_float4(v[4], v[5], v[6], v[7]);
-    } else if constexpr (ADJ) {
+    } else if constexpr (L == kWide) {
         *reinterpret_cast<uint4 *>(p + ca) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
     } else {
         *reinterpret_cast<uint2 *>(p + ca) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
@@ -94,12 +119,12 @@ struct Heads {
     int h0, h1;
 };
 
-// A warp takes a token and a run of its q and k heads; a head's dim / 8 units go
-// to as many lanes, 32 / units heads at a time.  Needs dim % 8 == 0, with halves
-// pairs % 4 == 0, heads aligned to four elements (ADJ: adjacent pairs, heads
-// aligned to eight).  POW2: dim / 8 is a power of two.
-template <typename T, bool ADJ, bool POW2>
-__global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const qmm_rotary_args a, const int heads_per_warp) {
+// A warp takes a token and a run of its q and k heads.  Needs dim % 8 == 0, with
+// halves pairs % 4 == 0, heads aligned as the layout says.  NORM: some weight is
+// given; POW2: dim / 8 is a power of two.
+template <typename T, Layout L, bool NORM, bool POW2>
+__global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qmm_rotary_args a, const int heads_per_warp) {
+    constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;  // heads a lane group has in flight
     const int units = a.dim >> 3, at_a_time = 32 / units;
     const int lane = threadIdx.x & 31, sub = lane / units, u = lane - sub * units;
     const uint32_t row = blockIdx.x * kWarps + (threadIdx.x >> 5);
@@ -107,60 +132,63 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const qmm_rotary_ar
     const uint32_t tokens = (uint32_t)a.tokens, batch = row / tokens, token = row - batch * tokens;
     const int first = blockIdx.y * heads_per_warp, last = first + heads_per_warp;
     const bool live = sub < at_a_time;
-    int ca = u * 8, cb = u * 8 + 4;
     const int pair = u * 4;
-    if (!ADJ && pair < a.pairs && !a.adjacent) ca = pair, cb = a.pairs + pair;
-    float cs[4], sn[4];
-    bool turned = false;
+    const int ca = L == kHalves && pair < a.pairs ? pair : u * 8, cb = L == kHalves && pair < a.pairs ? a.pairs + pair : u * 8 + 4;
     const float inv_dim = 1.0f / (float)a.dim;
+    float2 cs[2], sn[2];
+    bool turned = false;
 
-    auto run = [&](const Heads<T> &h, const T *weight) {
+    auto run = [&](const Heads<T> &h, const void *weight) {
         if (h.h0 >= h.h1) return;
         const T *src = h.src + (int64_t)(h.h0 + sub) * h.src_stride;
         T *dst = h.dst + (int64_t)(h.h0 + sub) * h.dst_stride;
         const int64_t src_step = at_a_time * h.src_stride, dst_step = at_a_time * h.dst_stride;
-        // out[even] = r (v[even] A - v[odd] B), out[odd] = r (v[even] C + v[odd] D): weight and turn in one factor
-        float fa[4], fb[4], fc[4], fd[4];
+        int left = live ? h.h1 - h.h0 - sub : 0;  // heads from this lane's on
+        // first = r (x A + y B), second = r (x C + y D): the norm's weights and the turn in one factor
+        float2 fa[2], fb[2], fc[2], fd[2];
         for (int hb = h.h0; hb < h.h1; hb += at_a_time * kAhead) {
             Runs<T> raw[kAhead];
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 raw[j] = Runs<T>{};
-                if (live && hb + j * at_a_time + sub < h.h1) raw[j] = load_runs<T, ADJ>(src + j * src_step, ca, cb);
+                if (j * at_a_time < left) raw[j] = load_runs<T, L>(src + j * src_step, ca, cb);
             }
-            if (!turned) {  // (after the first loads are on their way)
+            if (!turned) {  // (while the first heads are on their way)
                 turned = true;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    cs[i] = 1.0f, sn[i] = 0.0f;
-                    if (live && pair + i < a.pairs) pair_turn(a, batch, token, pair + i, &cs[i], &sn[i]);
+                for (int i = 0; i < 2; ++i) {
+                    cs[i] = twice(1.0f), sn[i] = twice(0.0f);
+                    if (live && pair + 2 * i < a.pairs) pair_turn(a, batch, token, pair + 2 * i, &cs[i].x, &sn[i].x);
+                    if (live && pair + 2 * i + 1 < a.pairs) pair_turn(a, batch, token, pair + 2 * i + 1, &cs[i].y, &sn[i].y);
                 }
             }
             if (hb == h.h0) {
-                float w[8];
+                float2 we[2] = {twice(1.0f), twice(1.0f)}, wo[2] = {twice(1.0f), twice(1.0f)};
+                if (NORM && weight && live) runs_to_pairs<T, L>(load_runs<T, L>(static_cast<const T *>(weight), ca, cb), we, wo);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = 1.0f;
-                if (weight && live) runs_to_f32(load_runs<T, ADJ>(weight, ca, cb), w);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float we = w[(ADJ || a.adjacent) ? 2 * i : i], wo = w[(ADJ || a.adjacent) ? 2 * i + 1 : i + 4];
-                    fa[i] = we * cs[i], fb[i] = wo * sn[i], fc[i] = we * sn[i], fd[i] = wo * cs[i];
+                for (int i = 0; i < 2; ++i) {
+                    fa[i] = mul_f32x2(we[i], cs[i]);
+                    fb[i] = mul_f32x2(wo[i], make_float2(-sn[i].x, -sn[i].y));
+                    fc[i] = mul_f32x2(we[i], sn[i]);
+                    fd[i] = mul_f32x2(wo[i], cs[i]);
                 }
             }
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
-                float v[8];
-                runs_to_f32(raw[j], v);
-                float r = 1.0f;
-                if (weight) {
-                    float s = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) s = fmaf(v[i], v[i], s);
+                if (hb + j * at_a_time >= h.h1) break;
+                float2 x[2], y[2];
+                runs_to_pairs<T, L>(raw[j], x, y);
+                if (NORM && weight) {
+                    float2 p = mul_f32x2(x[0], x[0]);
+                    p = fma_f32x2(x[1], x[1], p);
+                    p = fma_f32x2(y[0], y[0], p);
+                    p = fma_f32x2(y[1], y[1], p);
+                    float s = p.x + p.y;
                     if constexpr (POW2) {
 #pragma unroll
                         for (int o = 16; o > 0; o >>= 1)
                             if (o < units) s += __shfl_xor_sync(0xffffffffu, s, o);
-                    } else {
+                    } else {  // lanes u .. of the head's units, then the first one's sum
 #pragma unroll
                         for (int o = 1; o < 32; o <<= 1) {
                             if (o < units) {
@@ -170,36 +198,33 @@ __global__ void __launch_bounds__(kWarps * 32) rotary_kernel(const qmm_rotary_ar
                         }
                         s = __shfl_sync(0xffffffffu, s, lane - u);
                     }
-                    r = rsqrtf(s * inv_dim + a.eps);
-                }
-                float o[8];
-                if (ADJ || a.adjacent) {
+                    const float2 r = twice(rsqrtf(s * inv_dim + a.eps));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        o[2 * i] = r * (v[2 * i] * fa[i] - v[2 * i + 1] * fb[i]);
-                        o[2 * i + 1] = r * (v[2 * i] * fc[i] + v[2 * i + 1] * fd[i]);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        o[i] = r * (v[i] * fa[i] - v[i + 4] * fb[i]);
-                        o[i + 4] = r * (v[i] * fc[i] + v[i + 4] * fd[i]);
-                    }
+                    for (int q = 0; q < 2; ++q) x[q] = mul_f32x2(x[q], r), y[q] = mul_f32x2(y[q], r);
                 }
-                if (live && hb + j * at_a_time + sub < h.h1) store_runs<T, ADJ>(dst + j * dst_step, ca, cb, o);
+                if (j * at_a_time < left) {
+                    float2 oa[2], ob[2];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        oa[q] = fma_f32x2(x[q], fa[q], mul_f32x2(y[q], fb[q]));
+                        ob[q] = fma_f32x2(x[q], fc[q], mul_f32x2(y[q], fd[q]));
+                    }
+                    store_pairs<T, L>(dst + j * dst_step, ca, cb, oa, ob);
+                }
             }
             src += src_step * kAhead;
             dst += dst_step * kAhead;
+            left -= at_a_time * kAhead;
         }
     };
     run(Heads<T>{static_cast<const T *>(a.q) + batch * a.q_stride[0] + token * a.q_stride[1],
                  static_cast<T *>(a.q_out) + batch * a.q_out_stride[0] + token * a.q_out_stride[1], a.q_stride[2], a.q_out_stride[2],
                  first, min(last, a.q_heads)},
-        static_cast<const T *>(a.q_weight));
+        a.q_weight);
     run(Heads<T>{static_cast<const T *>(a.k) + batch * a.k_stride[0] + token * a.k_stride[1],
                  static_cast<T *>(a.k_out) + batch * a.k_out_stride[0] + token * a.k_out_stride[1], a.k_stride[2], a.k_out_stride[2],
                  max(first - a.q_heads, 0), min(last - a.q_heads, a.k_heads)},
-        static_cast<const T *>(a.k_weight));
+        a.k_weight);
 }
 
 // Any dim up to 256, any pairs, any alignment: lane l takes pairs l, l + 32, ...
@@ -286,13 +311,17 @@ static qmm_status launch(const qmm_rotary_args &a, bool fast, bool wide, cudaStr
     int per = (int)((heads + splits - 1) / splits);
     per = (per + at_a_time - 1) / at_a_time * at_a_time;
     const dim3 grid((unsigned)((rows + kWarps - 1) / kWarps), (unsigned)((heads + per - 1) / per), 1);
-    const bool pow2 = fast && (units & (units - 1)) == 0;
     if (grid.y > 65535) return fail(QMM_ERR_UNSUPPORTED, "rotary: %d heads are past the launch limits", heads);
+    const bool norm = a.q_weight || a.k_weight, pow2 = (units & (units - 1)) == 0;
+#define QMM_ROTARY(L)                                                                            \
+    (!norm  ? rotary_kernel<T, L, false, true><<<grid, kWarps * 32, 0, st>>>(a, per)             \
+     : pow2 ? rotary_kernel<T, L, true, true><<<grid, kWarps * 32, 0, st>>>(a, per)              \
+            : rotary_kernel<T, L, true, false><<<grid, kWarps * 32, 0, st>>>(a, per))
     if (!fast) rotary_any_kernel<T><<<grid, kWarps * 32, 0, st>>>(a, per);
-    else if (wide && pow2) rotary_kernel<T, true, true><<<grid, kWarps * 32, 0, st>>>(a, per);
-    else if (wide) rotary_kernel<T, true, false><<<grid, kWarps * 32, 0, st>>>(a, per);
-    else if (pow2) rotary_kernel<T, false, true><<<grid, kWarps * 32, 0, st>>>(a, per);
-    else rotary_kernel<T, false, false><<<grid, kWarps * 32, 0, st>>>(a, per);
+    else if (wide) QMM_ROTARY(kWide);
+    else if (a.adjacent) QMM_ROTARY(kAdjacent);
+    else QMM_ROTARY(kHalves);
+#undef QMM_ROTARY
     count_launch();
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? QMM_OK : cuda_fail(e, "rotary launch");
