@@ -102,7 +102,7 @@ __device__ __forceinline__ void request_residual(const CUtensorMap *tmap_res, co
 // through its staging buffer to y.
 __device__ __forceinline__ void chunk_finish(const Params &p, const CUtensorMap *tmap_y, const ChunkOut &o, const float *vec, uint32_t (&r)[32],
                                              int f0, int m0, bool res_tma) {
-    const int lane = threadIdx.x & 31, row = m0 + lane;
+    const int lane = threadIdx.x & 31;
     const float4 *const bias = reinterpret_cast<const float4 *>(vec), *const gate = bias + kChunk / 4;
     // Each step over all 32 features: its branch is taken once, and the exponentials overlap.
     float v[32];
@@ -138,26 +138,33 @@ __device__ __forceinline__ void chunk_finish(const Params &p, const CUtensorMap 
         }
     }
     auto cell = [&](int g) { return reinterpret_cast<uint4 *>(o.stage + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)); };
+    // This lane's feature of token t, where rows of y are not on 16-byte boundaries and a warp moves them one by one.
+    auto element = [&](int t) { return reinterpret_cast<uint16_t *>(o.stage + t * 64 + (((lane >> 3) ^ ((t >> 1) & 3)) << 4) + (lane & 7) * 2); };
+    const int rows = f0 + lane < p.n ? min(32, p.m - m0) : 0;
+    const int64_t at = (int64_t)m0 * p.n + f0 + lane;
+    if (p.ep.residual && !res_tma) {
+#pragma unroll 1
+        for (int t0 = 0; t0 < 32; t0 += 4) {
+            uint16_t w[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) w[t] = t0 + t < rows ? p.ep.residual[at + (int64_t)(t0 + t) * p.n] : 0;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) *element(t0 + t) = w[t];
+        }
+        __syncwarp();
+    }
     if (p.ep.residual) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {  // eight features: 16 bytes of this token's row
             float res[8];
-            if (res_tma) {
-                Vec8<Bf16> w;
-                w.w[0] = *cell(g);
-                vec8_to_f32(w, res);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int f = f0 + g * 8 + e;
-                    res[e] = row < p.m && f < p.n ? bf16_bits_to_f32(p.ep.residual[(int64_t)row * p.n + f]) : 0.0f;
-                }
-            }
+            Vec8<Bf16> w;
+            w.w[0] = *cell(g);
+            vec8_to_f32(w, res);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[g * 8 + e] = p.ep.res_mul ? res[e] * v[g * 8 + e] : res[e] + v[g * 8 + e];
         }
     }
-    if (!res_tma) {
+    if (p.tma_out && !res_tma) {
         if (lane == 0) bulk_wait_read<0>();  // the last store has left the buffer
         __syncwarp();
     }
@@ -174,10 +181,14 @@ __device__ __forceinline__ void chunk_finish(const Params &p, const CUtensorMap 
         }
     } else {
         __syncwarp();
-        const int rows = min(32, p.m - m0);
-        for (int t = 0; t < rows; ++t) {
-            const uint16_t w = *reinterpret_cast<const uint16_t *>(o.stage + t * 64 + (((lane >> 3) ^ ((t >> 1) & 3)) << 4) + (lane & 7) * 2);
-            if (f0 + lane < p.n) p.y[(int64_t)(m0 + t) * p.n + f0 + lane] = w;
+#pragma unroll 1
+        for (int t0 = 0; t0 < 32; t0 += 4) {
+            uint16_t w[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) w[t] = *element(t0 + t);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (t0 + t < rows) p.y[at + (int64_t)(t0 + t) * p.n] = w[t];
         }
         __syncwarp();
     }
