@@ -271,9 +271,10 @@ PyObject *qk_norm_rotary(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     });
 }
 
-// gated_norm(x, branch, post, post_weight, gate, residual_scale, pre, pre_weight, scale, shift, eps, quantize) -> (x', n) or (x', codes, scales)
+// gated_norm(x, branch, post, post_weight, gate, residual_scale, pre, pre_weight, scale, shift, eps, quantize, same)
+//   -> (x', n) or (x', codes, scales); same: x' is x itself
 PyObject *gated_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
-    ARITY(12)
+    ARITY(13)
     return guarded([&]() -> PyObject * {
         const at::Tensor *x = tensor(args[0]), *branch, *pw, *gate, *qw, *scale, *shift;
         if (!x || !optional_tensor(args[1], &branch) || !optional_tensor(args[3], &pw) || !optional_tensor(args[4], &gate) ||
@@ -284,7 +285,7 @@ PyObject *gated_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         a.residual_scale = (float)PyFloat_AsDouble(args[5]);
         a.pre = (int32_t)PyLong_AsLong(args[6]);
         a.eps = (float)PyFloat_AsDouble(args[10]);
-        const int quantize = PyObject_IsTrue(args[11]);
+        const int quantize = PyObject_IsTrue(args[11]), same = PyObject_IsTrue(args[12]);
         if (PyErr_Occurred()) return nullptr;
         if (a.post < 0 || a.pre < 0) Py_RETURN_NONE;
         const at::Device d = x->device();
@@ -323,9 +324,14 @@ PyObject *gated_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
             !vector(scale, true, &a.scale, &a.scale_stride) || !vector(shift, true, &a.shift, &a.shift_stride))
             Py_RETURN_NONE;
         a.vec_elem = elem < 0 ? 0 : elem;
-        at::Tensor xn = empty(x->sizes(), x->scalar_type(), d), n, scales;
-        a.x_out = xn.mutable_data_ptr();
-        a.x_out_stride = r.cols;
+        at::Tensor xn, n, scales;
+        if (same) {
+            xn = *x;
+        } else {
+            xn = empty(x->sizes(), x->scalar_type(), d);
+            a.x_out = xn.mutable_data_ptr();
+            a.x_out_stride = r.cols;
+        }
         if (quantize) {
             n = empty({r.rows, (r.cols + 31) / 32 * 16}, at::kByte, d);
             scales = empty({(r.rows + 127) / 128 * ((r.cols + 255) / 256) * 1024}, at::kByte, d);

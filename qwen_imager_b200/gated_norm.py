@@ -32,10 +32,12 @@ def gated_residual_norm(x: torch.Tensor, branch: Optional[torch.Tensor] = None, 
     [groups, 1, hidden]) for rows in `groups` equal runs, e.g. the sequences of
     a batch.  f32 inside, one rounding per output, n from the unrounded x'.
     x_out may be x or branch, n_out may be either too; quantize=True gives n as
-    an MxTensor."""
+    an MxTensor.  Without a branch and with residual_scale 1, x' is x itself
+    (nothing is written) unless x_out is given."""
+    same = branch is None and residual_scale == 1.0 and x_out is None  # x' would be a copy of x
     if x_out is None and n_out is None:
         made = _block.host().gated_norm(x, branch, _block.NORMS.get(post, -1), post_weight, gate, residual_scale,
-                                        _block.NORMS.get(pre, -1), pre_weight, scale, shift, eps, quantize)
+                                        _block.NORMS.get(pre, -1), pre_weight, scale, shift, eps, quantize, same)
         if made is not None:
             made = _block.checked(made)
             if not quantize:
@@ -60,7 +62,7 @@ def gated_residual_norm(x: torch.Tensor, branch: Optional[torch.Tensor] = None, 
         b_ptr, b_stride = b2.data_ptr(), b2.stride(0)
     if quantize and n_out is not None:
         raise bad_argument("n_out holds n in x's type; quantize=True returns it as an MxTensor")
-    x_new, xo = _output(x_out, x, shape, hidden, "x_out")
+    x_new, xo = (x, None) if same else _output(x_out, x, shape, hidden, "x_out")
     n_ptr = n_stride = c_ptr = s_ptr = 0
     if quantize:
         n_new = MxTensor.empty(rows, hidden, device, shape[:-1])
@@ -92,8 +94,8 @@ def gated_residual_norm(x: torch.Tensor, branch: Optional[torch.Tensor] = None, 
     (g, gs), (sc, ss), (sh, hs) = (_vector(v, dtype, hidden, groups, "modulation") for v in (gate, scale, shift))
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     _block.run("qmm_gated_residual_norm", device, _block.NORM.pack(
-        x2.data_ptr(), b_ptr, xo.data_ptr(), n_ptr, c_ptr, s_ptr, ptr(pw), ptr(qw), ptr(g), ptr(sh), ptr(sc), rows, hidden,
-        x2.stride(0), b_stride, xo.stride(0), n_stride, gs, hs, ss, groups, x_elem, b_elem, _block.ELEMS[dtype], post_kind,
+        x2.data_ptr(), b_ptr, ptr(xo), n_ptr, c_ptr, s_ptr, ptr(pw), ptr(qw), ptr(g), ptr(sh), ptr(sc), rows, hidden,
+        x2.stride(0), b_stride, 0 if xo is None else xo.stride(0), n_stride, gs, hs, ss, groups, x_elem, b_elem, _block.ELEMS[dtype], post_kind,
         pre_kind, residual_scale, eps))
     return x_new, n_new
 
