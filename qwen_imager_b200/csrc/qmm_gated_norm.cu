@@ -3,18 +3,19 @@
 //   x' = residual_scale * x + gate * h
 //   n  = norm_pre(x') * pre_weight * (1 + scale) + shift
 // HBM-bound: x and branch are read once, x' and n (or its MXFP4 codes) written
-// once.  A CTA takes a row at a time and keeps it in registers (eight columns a
-// vector, up to four vectors a thread), so mean and variance are two passes over
-// registers, and each statistic costs one shuffle tree, one shared slot a warp and one
-// barrier.  The grid is what is resident at once, consecutive rows to a CTA; it loads
-// its next row while it works on this one.  Weights and modulation enter a row as three vectors, A =
-// post_weight * gate, S = pre_weight * (1 + scale) and H = shift, formed once a CTA
-// (and group) in shared memory, and arithmetic goes two columns an instruction:
+// once.  A row stays in the registers of a warp (up to 1024 columns, several rows a
+// CTA) or of a CTA, eight columns a vector, up to four vectors a thread, so mean and
+// variance are two passes over registers, and each statistic costs one shuffle tree
+// and, in a CTA, one shared slot a warp and one barrier.  The grid is what is resident
+// at once, consecutive rows to a warp or CTA; it loads its next row while it works on
+// this one.  Weights and modulation enter a row as three vectors, A = post_weight *
+// gate, S = pre_weight * (1 + scale) and H = shift, formed once (and again where the
+// group changes) in shared memory, and arithmetic goes two columns an instruction:
 // with the vectors loaded and converted row by row the kernel was bound by its
-// instructions (16896 x 3072 bf16: 116 us).
-// Rows that are not 16-byte aligned take a kernel with columns dealt out one by
-// one (thread t holds columns t, t + T, ...), which keeps accesses of a warp
-// consecutive; so do rows past 16384 columns, whose vectors do not fit.
+// instructions (16896 x 3072 bf16: 116 us against 85).
+// Rows that are not 16-byte aligned deal their columns out one by one (thread t
+// holds columns t, t + T, ...), which keeps accesses of a warp consecutive.  Rows past
+// 16384 columns, whose vectors do not fit, take a kernel without them.
 #include <algorithm>
 #include <type_traits>
 
@@ -68,8 +69,10 @@ struct RowSum {
     float (&red)[4][SLOTS];
     int set = 0;
     __device__ __forceinline__ RowSum(float (&r)[4][SLOTS]) : red(r) {
-        for (int i = threadIdx.x; i < 4 * SLOTS; i += blockDim.x) (&red[0][0])[i] = 0.0f;
-        __syncthreads();
+        if (blockDim.x > 32) {
+            for (int i = threadIdx.x; i < 4 * SLOTS; i += blockDim.x) (&red[0][0])[i] = 0.0f;
+            __syncthreads();
+        }
     }
     __device__ __forceinline__ float operator()(float s) {
 #pragma unroll
@@ -116,88 +119,172 @@ __device__ __forceinline__ void normalise(float (&v)[VPT][8], int kind, float in
         for (int q = 0; q < 8; ++q) v[i][q] *= r;
 }
 
-// x and branch rows, and outputs, 16-byte aligned; hidden a multiple of 8.
-template <typename T, int BBYTES, int VPT, int MAXT, int MINB>
-__global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group, const uint32_t rows_per_cta,
-                                                                  const bool vec_aligned) {
-    extern __shared__ float4 vectors[];  // A, S, H: threads * VPT * 8 columns each (0 past the row), every thread's its own
+// MXFP4 of one column a lane: a warp's 32 lanes hold one block, column c this lane's.
+__device__ __forceinline__ void encode_lane(const qmm_gated_norm_args &a, int64_t row, int c, float v, int64_t pitch, int64_t tiles) {
+    const int lane = threadIdx.x & 31;
+    uint32_t m = __float_as_uint(v) & 0x7FFFFFFFu;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t e = mx4_scale_code(m);
+    const float one[8] = {v * mx4_inverse_scale(e), 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    uint32_t word = e == 255u ? 0u : (mx4_pack8(one) & 15u) << (4 * (lane & 7));
+    word |= __shfl_xor_sync(0xffffffffu, word, 1);
+    word |= __shfl_xor_sync(0xffffffffu, word, 2);
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    if ((lane & 7) == 0 && c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = word;
+    const int64_t b = c / kMxBlock;
+    if (lane == 0 && b < tiles * 4) a.n_scales[mx4_scale_offset(row, b, tiles)] = (uint8_t)e;
+}
+
+// Eight elements of one thread's row: as vectors (VEC) or one by one.
+template <typename T, int BYTES, bool VEC>
+struct Held {
+    Raw8<BYTES> v;
+};
+template <typename T, int BYTES>
+struct Held<T, BYTES, false> {
+    uint32_t e[8];  // bits of each element
+};
+
+// blockDim.x threads a row, blockDim.y rows side by side (more than one only with 32
+// threads a row).  VEC: x and branch rows, and outputs, 16-byte aligned, hidden a
+// multiple of 8.
+template <typename T, int BBYTES, int VPT, int MAXT, int MINB, bool VEC>
+__global__ void __launch_bounds__(MAXT, MINB)
+    gated_norm_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group, const uint32_t rows_each, const bool vec_aligned) {
+    extern __shared__ float4 shared_vectors[];  // A, S, H of each row side by side: threads * VPT * 8 columns (0 past the row), every thread's its own
     __shared__ __align__(16) float red[4][MAXT / 32];
     RowSum<MAXT / 32> row_sum{red};
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
     const int hidden = (int)a.hidden;
     const float inv_hidden = 1.0f / (float)hidden;
-    auto column = [&](int i) { return (i * threads + tid) * 8; };
+    auto column = [&](int i, int q) { return VEC ? (i * threads + tid) * 8 + q : (i * 8 + q) * threads + tid; };
+    auto valid = [&](int i, int q) { return column(i, VEC ? 0 : q) < hidden; };
     constexpr int XB = (int)sizeof(T);
     const bool f16_branch = a.branch_elem == QMM_ELEM_F16;
     const int span = threads * VPT * 2;  // float4 a vector
+    float4 *const vectors = shared_vectors + threadIdx.y * 3 * span;
 
-    Raw8<XB> rx[VPT];
-    Raw8<BBYTES> rb[VPT];
+    Held<T, XB, VEC> rx[VPT];
+    Held<T, BBYTES, VEC> rb[VPT];
     auto fetch = [&](int64_t row) {
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            rx[i] = Raw8<XB>{};
-            rb[i] = Raw8<BBYTES>{};
-            if (column(i) < hidden) {
-                rx[i] = load_raw8<XB>(a.x, row * a.x_stride + column(i));
-                if (a.branch) rb[i] = load_raw8<BBYTES>(a.branch, row * a.branch_stride + column(i));
+            rx[i] = {};
+            rb[i] = {};
+            if constexpr (VEC) {
+                if (valid(i, 0)) {
+                    rx[i].v = load_raw8<XB>(a.x, row * a.x_stride + column(i, 0));
+                    if (a.branch) rb[i].v = load_raw8<BBYTES>(a.branch, row * a.branch_stride + column(i, 0));
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    if (valid(i, q)) {
+                        const int64_t c = column(i, q);
+                        rx[i].e[q] = XB == 4 ? static_cast<const uint32_t *>(a.x)[row * a.x_stride + c] : static_cast<const uint16_t *>(a.x)[row * a.x_stride + c];
+                        if (a.branch)
+                            rb[i].e[q] = BBYTES == 4 ? static_cast<const uint32_t *>(a.branch)[row * a.branch_stride + c]
+                                                     : static_cast<const uint16_t *>(a.branch)[row * a.branch_stride + c];
+                    }
+                }
             }
         }
     };
+    auto unpack = [&](const auto &held, bool f16, float2 (&v)[4]) {
+        constexpr bool kWide = std::is_same<decltype(held), const Held<T, 4, VEC> &>::value;
+        float w[8];
+        (void)kWide;
+        if constexpr (VEC) {
+            raw8_to_f32(held.v, f16, w);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                w[q] = kWide ? __uint_as_float(held.e[q]) : f16 ? elem_to_f32(F16{(uint16_t)held.e[q]}) : elem_to_f32(Bf16{(uint16_t)held.e[q]});
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = make_float2(w[2 * q], w[2 * q + 1]);
+    };
     auto store = [&](void *p, int64_t base, const float2 (&v)[VPT][4]) {
+        T *const o = static_cast<T *>(p) + base;
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            if (column(i) < hidden) {
-                const float w[8] = {v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y, v[i][2].x, v[i][2].y, v[i][3].x, v[i][3].y};
-                store_vec8(static_cast<T *>(p) + base + column(i), w);
+            const float w[8] = {v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y, v[i][2].x, v[i][2].y, v[i][3].x, v[i][3].y};
+            if constexpr (VEC) {
+                if (valid(i, 0)) store_vec8(o + column(i, 0), w);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (valid(i, q)) o[column(i, q)] = elem_from_f32<T>(w[q]);
             }
         }
     };
     // This thread's eight columns of vector `which`.
-    auto mine = [&](int which, int i) { return vectors + which * span + (i * threads + tid) * 2; };
+    auto mine = [&](int which, int i) { return vectors + which * span + i * threads * 2 + tid; };
     auto vec8 = [&](int which, int i, float2 (&w)[4]) {
         const float4 *q = mine(which, i);
-        const float4 lo = q[0], hi = q[1];
+        const float4 lo = q[0], hi = q[threads];
         w[0] = make_float2(lo.x, lo.y), w[1] = make_float2(lo.z, lo.w), w[2] = make_float2(hi.x, hi.y), w[3] = make_float2(hi.z, hi.w);
     };
-    // Forms this thread's columns of A, S and H; every load is on its way before the first is used.
+    // Forms this thread's columns of A, S and H.
     auto take_vectors = [&](uint32_t group) {
-#pragma unroll
+        const int64_t gate = group * a.gate_stride, scale = group * a.scale_stride, shift = group * a.shift_stride;
+#pragma unroll 1
         for (int i = 0; i < VPT; ++i) {
-            const int c = column(i);
-            const bool in = c < hidden;
-            const void *const src[5] = {a.post_weight, a.gate, a.pre_weight, a.scale, a.shift};
-            const int64_t at[5] = {c, group * a.gate_stride + c, c, group * a.scale_stride + c, group * a.shift_stride + c};
-            Raw8<4> raw[5];
-            float w[5][8];
-            const float one = in ? 1.0f : 0.0f;
-            if (vec_aligned) {
+            auto put = [&](int k, const float (&f)[8]) {
+                float4 *o = mine(k, i);
+                o[0] = make_float4(f[0], f[1], f[2], f[3]);
+                o[threads] = make_float4(f[4], f[5], f[6], f[7]);
+            };
+            if (VEC && vec_aligned) {  // every load is on its way before the first is used
+                const bool in = valid(i, 0);
+                const int c = column(i, 0);
+                auto raw = [&](const void *p, int64_t at) {
+                    Raw8<4> r{};
+                    if (in && p) {
+                        if (a.vec_elem == QMM_ELEM_F32) r = load_raw8<4>(p, at + c);
+                        else r.w[0] = load_raw8<2>(p, at + c).w[0];
+                    }
+                    return r;
+                };
+                auto values = [&](const Raw8<4> &r, const void *p, float none, float (&w)[8]) {
+                    if (a.vec_elem == QMM_ELEM_F32) raw8_to_f32(r, false, w);
+                    else raw8_to_f32(Raw8<2>{{r.w[0]}}, a.vec_elem == QMM_ELEM_F16, w);
+                    if (!p) {
 #pragma unroll
-                for (int k = 0; k < 5; ++k) {
-                    raw[k] = Raw8<4>{};
-                    if (in && src[k]) {
-                        if (a.vec_elem == QMM_ELEM_F32) raw[k] = load_raw8<4>(src[k], at[k]);
-                        else raw[k].w[0] = load_raw8<2>(src[k], at[k]).w[0];
+                        for (int q = 0; q < 8; ++q) w[q] = none;
+                    }
+                };
+                const Raw8<4> r0 = raw(a.post_weight, 0), r1 = raw(a.gate, gate), r2 = raw(a.pre_weight, 0), r3 = raw(a.scale, scale), r4 = raw(a.shift, shift);
+                const float one = in ? 1.0f : 0.0f;
+                float f[8], w[8];
+                values(r0, a.post_weight, one, f);
+                values(r1, a.gate, 1.0f, w);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) f[q] *= w[q];
+                put(0, f);
+                values(r2, a.pre_weight, one, f);
+                values(r3, a.scale, 0.0f, w);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) f[q] = fmaf(f[q], w[q], f[q]);
+                put(1, f);
+                values(r4, a.shift, 0.0f, f);
+                put(2, f);
+            } else {
+                float f[3][8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    f[0][q] = f[1][q] = f[2][q] = 0.0f;
+                    if (valid(i, q)) {
+                        const int64_t c = column(i, q);
+                        f[0][q] = (a.post_weight ? load_elem(a.post_weight, a.vec_elem, c) : 1.0f) * (a.gate ? load_elem(a.gate, a.vec_elem, gate + c) : 1.0f);
+                        const float w = a.pre_weight ? load_elem(a.pre_weight, a.vec_elem, c) : 1.0f;
+                        f[1][q] = a.scale ? fmaf(w, load_elem(a.scale, a.vec_elem, scale + c), w) : w;
+                        if (a.shift) f[2][q] = load_elem(a.shift, a.vec_elem, shift + c);
                     }
                 }
 #pragma unroll
-                for (int k = 0; k < 5; ++k) {
-                    if (a.vec_elem == QMM_ELEM_F32) raw8_to_f32(raw[k], false, w[k]);
-                    else raw8_to_f32(Raw8<2>{{raw[k].w[0]}}, a.vec_elem == QMM_ELEM_F16, w[k]);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 5; ++k)
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) w[k][q] = in && src[k] ? load_elem(src[k], a.vec_elem, at[k] + q) : 0.0f;
-            }
-            float *const fa = reinterpret_cast<float *>(mine(0, i)), *const fs = reinterpret_cast<float *>(mine(1, i)), *const fh = reinterpret_cast<float *>(mine(2, i));
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const float pw = src[0] ? w[0][q] : one, g = src[1] ? w[1][q] : 1.0f, qw = src[2] ? w[2][q] : one;
-                fa[q] = pw * g;
-                fs[q] = fmaf(qw, w[3][q], qw);
-                fh[q] = w[4][q];
+                for (int k = 0; k < 3; ++k) put(k, f[k]);
             }
         }
     };
@@ -210,11 +297,10 @@ __global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_
             for (int q = 0; q < 4; ++q) s = add_f32x2(s, v[i][q]);
         const float mean = row_sum(s.x + s.y) * inv_hidden;
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const float2 m = twice(column(i) < hidden ? -mean : 0.0f);
+        for (int i = 0; i < VPT; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[i][q] = add_f32x2(v[i][q], m);
-        }
+            for (int q = 0; q < 4; ++q)
+                v[i][q] = add_f32x2(v[i][q], make_float2(valid(i, 2 * q) ? -mean : 0.0f, valid(i, 2 * q + 1) ? -mean : 0.0f));
     };
     auto rms = [&](const float2 (&v)[VPT][4]) {
         float2 s = twice(0.0f);
@@ -227,8 +313,8 @@ __global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_
     const int64_t pitch = mx4_pitch(hidden), tiles = mx4_scale_tiles(hidden);
 
     pdl_launch_dependents();  // a product behind this pass sets itself up meanwhile; it waits for the grid before it reads
-    const uint32_t first = blockIdx.x * rows_per_cta, last = min(first + rows_per_cta, (uint32_t)a.rows);
-    fetch(first);
+    const uint32_t first = (blockIdx.x * blockDim.y + threadIdx.y) * rows_each, last = min(first + rows_each, (uint32_t)a.rows);
+    if (first < last) fetch(first);
     uint32_t group = UINT32_MAX;
     for (uint32_t row = first; row < last; ++row) {
         if (row / rows_per_group != group) {
@@ -238,13 +324,8 @@ __global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_
         float2 x[VPT][4], h[VPT][4];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            float w[8];
-            raw8_to_f32(rx[i], std::is_same<T, F16>::value, w);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) x[i][q] = make_float2(w[2 * q], w[2 * q + 1]);
-            raw8_to_f32(rb[i], f16_branch, w);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) h[i][q] = make_float2(w[2 * q], w[2 * q + 1]);
+            unpack(rx[i], std::is_same<T, F16>::value, x[i]);
+            unpack(rb[i], f16_branch, h[i]);
         }
         if (row + 1 < last) fetch((int64_t)row + 1);
         const float2 c2 = twice(a.residual_scale);
@@ -280,33 +361,40 @@ __global__ void __launch_bounds__(MAXT, MINB) gated_norm_kernel(const qmm_gated_
             store(a.n_out, row * a.n_out_stride, x);
             continue;
         }
-        // MXFP4: columns past the row are zeros of its last block (their S and H are 0).
+        // MXFP4: columns past the row are zeros of its last block.
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            const int c = column(i);
             float w[8] = {x[i][0].x, x[i][0].y, x[i][1].x, x[i][1].y, x[i][2].x, x[i][2].y, x[i][3].x, x[i][3].y};
-            if (c >= hidden) {  // (0 times an infinite or NaN statistic)
 #pragma unroll
-                for (int q = 0; q < 8; ++q) w[q] = 0.0f;
+            for (int q = 0; q < 8; ++q)
+                if (!valid(i, q)) w[q] = 0.0f;  // (0 times an infinite or NaN statistic)
+            if constexpr (VEC) {
+                const int c = column(i, 0);
+                uint32_t codes;
+                const uint32_t e = mx4_encode8(w, &codes);
+                if (c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = codes;
+                uint32_t word = e << (8 * ((lane >> 2) & 3));
+                word |= __shfl_xor_sync(0xffffffffu, word, 4);
+                word |= __shfl_xor_sync(0xffffffffu, word, 8);
+                const int64_t b = c / kMxBlock;
+                if ((lane & 15) == 0 && b < tiles * 4) *reinterpret_cast<uint32_t *>(a.n_scales + mx4_scale_offset(row, b, tiles)) = word;
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    if (column(i, q) - lane >= tiles * 128) continue;  // the same in the whole warp
+                    encode_lane(a, row, column(i, q), w[q], pitch, tiles);
+                }
             }
-            uint32_t codes;
-            const uint32_t e = mx4_encode8(w, &codes);
-            if (c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = codes;
-            uint32_t word = e << (8 * ((lane >> 2) & 3));
-            word |= __shfl_xor_sync(0xffffffffu, word, 4);
-            word |= __shfl_xor_sync(0xffffffffu, word, 8);
-            const int64_t b = c / kMxBlock;
-            if ((lane & 15) == 0 && b < tiles * 4) *reinterpret_cast<uint32_t *>(a.n_scales + mx4_scale_offset(row, b, tiles)) = word;
         }
     }
 }
 
-// Any alignment and width.
+// Any alignment and width, nothing kept between rows.
 template <typename T, int VPT, int MAXT>
 __global__ void __launch_bounds__(MAXT) gated_norm_any_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group) {
     __shared__ __align__(16) float red[4][MAXT / 32];
     RowSum<MAXT / 32> row_sum{red};
-    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
+    const int tid = threadIdx.x, threads = blockDim.x;
     const int64_t row = blockIdx.x;
     const int hidden = (int)a.hidden;
     const int64_t group = (uint32_t)row / rows_per_group;
@@ -359,28 +447,12 @@ __global__ void __launch_bounds__(MAXT) gated_norm_any_kernel(const qmm_gated_no
         store(a.n_out, row * a.n_out_stride, x);
         return;
     }
-    // MXFP4: a warp's 32 lanes hold one block; columns past the row are zeros of its last block.
+    // MXFP4: columns past the row are zeros of its last block.
     const int64_t pitch = mx4_pitch(hidden), tiles = mx4_scale_tiles(hidden);
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
+    for (int i = 0; i < VPT; ++i)
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const int c = column(i, q);
-            const float v = c < hidden ? x[i][q] : 0.0f;
-            uint32_t m = __float_as_uint(v) & 0x7FFFFFFFu;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const uint32_t e = mx4_scale_code(m);
-            const float one[8] = {v * mx4_inverse_scale(e), 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            uint32_t word = e == 255u ? 0u : (mx4_pack8(one) & 15u) << (4 * (lane & 7));
-            word |= __shfl_xor_sync(0xffffffffu, word, 1);
-            word |= __shfl_xor_sync(0xffffffffu, word, 2);
-            word |= __shfl_xor_sync(0xffffffffu, word, 4);
-            if ((lane & 7) == 0 && c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = word;
-            const int64_t b = c / kMxBlock;
-            if (lane == 0 && b < tiles * 4) a.n_scales[mx4_scale_offset(row, b, tiles)] = (uint8_t)e;
-        }
-    }
+        for (int q = 0; q < 8; ++q) encode_lane(a, row, column(i, q), valid(i, q) ? x[i][q] : 0.0f, pitch, tiles);
 }
 
 // Threads a row: whole warps, the fewest that hold it in VPT vectors each.
@@ -390,50 +462,54 @@ static unsigned threads_for(int64_t hidden) {
     return (unsigned)(((vectors + VPT - 1) / VPT + 31) / 32 * 32);
 }
 
-template <typename T, int BBYTES, int VPT, int MAXT, int MINB>
+template <typename T, int BBYTES, int VPT, int MAXT, int MINB, bool VEC>
 static cudaError_t launch_rows(const qmm_gated_norm_args &a, uint32_t rpg, bool vec_aligned, cudaStream_t st) {
-    auto kernel = gated_norm_kernel<T, BBYTES, VPT, MAXT, MINB>;
+    auto kernel = gated_norm_kernel<T, BBYTES, VPT, MAXT, MINB, VEC>;
     const unsigned threads = threads_for<VPT>(a.hidden);
-    const size_t smem = (size_t)threads * VPT * 8 * 4 * 3;
-    static int resident[64][33] = {};  // CTAs an SM by device and warps
+    const dim3 block(threads, threads == 32 ? 4 : 1, 1);
+    const size_t smem = (size_t)threads * block.y * VPT * 8 * 4 * 3;
+    static int resident[64][33] = {};  // CTAs an SM by device and warps a row
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) dev = 0;
     int &n = resident[dev][threads / 32];
     if (n == 0) {
         int m = 0;
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAXT * VPT * 8 * 4 * 3);
-        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&m, kernel, (int)threads, smem);
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&m, kernel, (int)(threads * block.y), smem);
         if (e != cudaSuccess) return e;
         n = std::max(1, m);
     }
-    // Consecutive rows to a CTA: few of them cross into another group's vectors.
-    const int64_t per = (a.rows + (int64_t)sm_count() * n - 1) / ((int64_t)sm_count() * n);
-    kernel<<<(unsigned)((a.rows + per - 1) / per), threads, smem, st>>>(a, rpg, (uint32_t)per, vec_aligned);
+    // Consecutive rows to a warp or CTA: few of them cross into another group's vectors.
+    const int64_t places = (int64_t)sm_count() * n * block.y, each = (a.rows + places - 1) / places;
+    const int64_t used = (a.rows + each - 1) / each;
+    kernel<<<(unsigned)((used + block.y - 1) / block.y), block, smem, st>>>(a, rpg, (uint32_t)each, vec_aligned);
     return cudaGetLastError();
 }
 
-template <typename T, int BBYTES>
+template <typename T, int BBYTES, bool VEC>
 static cudaError_t launch_fast(const qmm_gated_norm_args &a, uint32_t rpg, bool vec_aligned, cudaStream_t st) {
-    if (a.hidden <= 2048) return launch_rows<T, BBYTES, 1, 256, 4>(a, rpg, vec_aligned, st);
-    if (a.hidden <= 4096) return launch_rows<T, BBYTES, 2, 256, 3>(a, rpg, vec_aligned, st);
-    if (a.hidden <= 8192) return launch_rows<T, BBYTES, 4, 256, 1>(a, rpg, vec_aligned, st);
-    return launch_rows<T, BBYTES, 4, 512, 1>(a, rpg, vec_aligned, st);
+    // A warp a row where its lanes hold it; then a CTA, with as many vectors a thread as
+    // its registers allow at 12 warps an SM or more (B200, 16896 x 2048 bf16: two vectors
+    // a thread 70 us, one 77).
+    constexpr bool W = sizeof(T) == 4 || BBYTES == 4 || !VEC;  // more registers a vector
+    if (a.hidden <= 256) return launch_rows<T, BBYTES, 1, 256, W ? 3 : 4, VEC>(a, rpg, vec_aligned, st);
+    if (a.hidden <= 512) return launch_rows<T, BBYTES, 2, 256, W ? 2 : 3, VEC>(a, rpg, vec_aligned, st);
+    if (VEC && a.hidden <= 1024) return launch_rows<T, BBYTES, 4, 256, 1, true>(a, rpg, vec_aligned, st);
+    if (a.hidden <= 4096) return launch_rows<T, BBYTES, 2, 256, W ? 2 : 3, VEC>(a, rpg, vec_aligned, st);
+    if (VEC && a.hidden <= 8192) return launch_rows<T, BBYTES, 4, 256, 1, true>(a, rpg, vec_aligned, st);
+    if (!VEC && a.hidden <= 8192) return launch_rows<T, BBYTES, 2, 512, 1, false>(a, rpg, vec_aligned, st);
+    return launch_rows<T, BBYTES, 4, 512, 1, VEC>(a, rpg, vec_aligned, st);
 }
 
 template <typename T>
-static cudaError_t launch_any(const qmm_gated_norm_args &a, uint32_t rpg, cudaStream_t st) {
-    const unsigned grid = (unsigned)a.rows;
-    if (a.hidden <= 1024) gated_norm_any_kernel<T, 1, 128><<<grid, threads_for<1>(a.hidden), 0, st>>>(a, rpg);
-    else if (a.hidden <= 4096) gated_norm_any_kernel<T, 2, 256><<<grid, threads_for<2>(a.hidden), 0, st>>>(a, rpg);
-    else if (a.hidden <= 16384) gated_norm_any_kernel<T, 4, 512><<<grid, threads_for<4>(a.hidden), 0, st>>>(a, rpg);
-    else gated_norm_any_kernel<T, 4, 1024><<<grid, threads_for<4>(a.hidden), 0, st>>>(a, rpg);
-    return cudaGetLastError();
-}
-
-template <typename T>
-static cudaError_t launch(const qmm_gated_norm_args &a, bool fast, bool vec_aligned, uint32_t rpg, cudaStream_t st) {
-    if (!fast) return launch_any<T>(a, rpg, st);
-    return a.branch_elem == QMM_ELEM_F32 ? launch_fast<T, 4>(a, rpg, vec_aligned, st) : launch_fast<T, 2>(a, rpg, vec_aligned, st);
+static cudaError_t launch(const qmm_gated_norm_args &a, bool vec, bool vec_aligned, uint32_t rpg, cudaStream_t st) {
+    if (a.hidden > 16384) {
+        gated_norm_any_kernel<T, 4, 1024><<<(unsigned)a.rows, threads_for<4>(a.hidden), 0, st>>>(a, rpg);
+        return cudaGetLastError();
+    }
+    const bool wide_branch = a.branch_elem == QMM_ELEM_F32;
+    if (vec) return wide_branch ? launch_fast<T, 4, true>(a, rpg, vec_aligned, st) : launch_fast<T, 2, true>(a, rpg, vec_aligned, st);
+    return wide_branch ? launch_fast<T, 4, false>(a, rpg, vec_aligned, st) : launch_fast<T, 2, false>(a, rpg, vec_aligned, st);
 }
 
 }  // namespace gnorm
@@ -529,7 +605,7 @@ extern "C" qmm_status qmm_gated_residual_norm(const qmm_gated_norm_args *p, void
     };
     const bool vec_aligned = aligned_vec(a.post_weight, 0) && aligned_vec(a.pre_weight, 0) && aligned_vec(a.gate, a.gate_stride) &&
                              aligned_vec(a.shift, a.shift_stride) && aligned_vec(a.scale, a.scale_stride);
-    const bool vec = a.hidden % 8 == 0 && a.hidden <= 16384 && aligned(a.x, a.x_stride, xs) && aligned(a.branch, a.branch_stride, bs) &&
+    const bool vec = a.hidden % 8 == 0 && aligned(a.x, a.x_stride, xs) && aligned(a.branch, a.branch_stride, bs) &&
                      aligned(a.x_out, a.x_out_stride, xs) && aligned(a.n_out, a.n_out_stride, xs);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const uint32_t rpg = (uint32_t)(a.rows / a.groups);

@@ -73,23 +73,6 @@ __device__ __forceinline__ void mx4_unpack8(uint32_t w, float (&v)[8]) {
     }
 }
 
-// Four lanes (aligned) hold a block of 32 values: the block's scale code, and
-// this lane's eight codes.  Called by the whole warp.
-__device__ __forceinline__ uint32_t mx4_encode8(float (&v)[8], uint32_t *codes) {
-    uint32_t a = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
-    a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
-    const uint32_t e = mx4_scale_code(a);
-    const float inv = mx4_inverse_scale(e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= inv;
-    const uint32_t w = mx4_pack8(v);
-    *codes = e == 255u ? 0u : w;
-    return e;
-}
-
 __device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
     uint64_t d;
     asm("{\n\t.reg .b64 ra, rb;\n\t"
@@ -101,6 +84,32 @@ __device__ __forceinline__ float2 mul_f32x2(float2 a, float2 b) {
     return make_float2(__uint_as_float(static_cast<uint32_t>(d)), __uint_as_float(static_cast<uint32_t>(d >> 32)));
 }
 __device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+
+// The larger magnitude; NaN if either is.
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+
+// Four lanes (aligned) hold a block of 32 values: the block's scale code, and
+// this lane's eight codes.  Called by the whole warp.
+__device__ __forceinline__ uint32_t mx4_encode8(float (&v)[8], uint32_t *codes) {
+    float m = max_abs(max_abs(max_abs(v[0], v[1]), max_abs(v[2], v[3])), max_abs(max_abs(v[4], v[5]), max_abs(v[6], v[7])));
+    m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const uint32_t e = mx4_scale_code(__float_as_uint(m) & 0x7FFFFFFFu);
+    const float2 inv = twice(mx4_inverse_scale(e));
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const float2 t = mul_f32x2(make_float2(v[i], v[i + 1]), inv);
+        v[i] = t.x;
+        v[i + 1] = t.y;
+    }
+    const uint32_t w = mx4_pack8(v);
+    *codes = e == 255u ? 0u : w;
+    return e;
+}
 
 // ---------------------------------------------------------------- elements
 // Typed loads and stores of the block operators (T: uint16_t tag types below
