@@ -3,7 +3,7 @@
 //   x' = residual_scale * x + gate * h
 //   n  = norm_pre(x') * pre_weight * (1 + scale) + shift
 // HBM-bound: x and branch are read once, x' and n (or its MXFP4 codes) written
-// once.  A row stays in the registers of a warp (up to 1024 columns, several rows a
+// once.  A row stays in the registers of a warp (up to 512 columns, several rows a
 // CTA) or of a CTA, eight columns a vector, up to four vectors a thread, so mean and
 // variance are two passes over registers, and each statistic costs one shuffle tree
 // and, in a CTA, one shared slot a warp and one barrier.  The grid is what is resident
@@ -494,9 +494,8 @@ static cudaError_t launch_fast(const qmm_gated_norm_args &a, uint32_t rpg, bool 
     constexpr bool W = sizeof(T) == 4 || BBYTES == 4 || !VEC;  // more registers a vector
     if (a.hidden <= 256) return launch_rows<T, BBYTES, 1, 256, W ? 3 : 4, VEC>(a, rpg, vec_aligned, st);
     if (a.hidden <= 512) return launch_rows<T, BBYTES, 2, 256, W ? 2 : 3, VEC>(a, rpg, vec_aligned, st);
-    if (VEC && a.hidden <= 1024) return launch_rows<T, BBYTES, 4, 256, 1, true>(a, rpg, vec_aligned, st);
     if (a.hidden <= 4096) return launch_rows<T, BBYTES, 2, 256, W ? 2 : 3, VEC>(a, rpg, vec_aligned, st);
-    if (VEC && a.hidden <= 8192) return launch_rows<T, BBYTES, 4, 256, 1, true>(a, rpg, vec_aligned, st);
+    if (VEC && a.hidden <= 8192) return launch_rows<T, BBYTES, 4, 256, W ? 1 : 2, true>(a, rpg, vec_aligned, st);
     if (!VEC && a.hidden <= 8192) return launch_rows<T, BBYTES, 2, 512, 1, false>(a, rpg, vec_aligned, st);
     return launch_rows<T, BBYTES, 4, 512, 1, VEC>(a, rpg, vec_aligned, st);
 }
