@@ -20,6 +20,11 @@
 // accumulators, so a tile's epilogue overlaps the next tile's main loop.  Scale
 // slots in tensor memory are tied to the shared-memory stages: a stage refilled
 // means that the MMAs that read its slot are complete.  Every wait is bounded.
+//
+// The one-CTA kernel runs where pairs (below) would leave SMs idle and k need not be
+// split (qmm_mx4_small.cu): B200, 512 x 3072 -> 3072 in 10.5 us.  At 128 x 192 its loads
+// (43 KB a stage) bound it: 4352 x 12288 -> 3072 takes 90 us here, 72 without the loads,
+// 74 on pairs.
 #include <algorithm>
 #include <climits>
 

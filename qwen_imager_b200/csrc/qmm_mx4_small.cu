@@ -11,6 +11,11 @@
 // weight is on its way (a warp a row of 256 columns: eight columns a lane, four lanes a
 // block), writing codes and scales straight into the stage's operand layout; an x that
 // is MXFP4 already comes by TMA instead.  The same warps then run the epilogue.
+//
+// HBM-bound where the weight is large, latency-bound where it is not.  B200, back to
+// back: 1 x 3072 -> 18432 7.1 us (30 MB: 4.6 us of HBM, the rest is the launch, the first
+// stage's arrival and the last tile's epilogue), 1 x 12288 -> 3072 7.6 us, 128 x 3072 ->
+// 12288 10.7 us, 8 x 512 -> 512 3.5 us.
 #include <algorithm>
 #include <cstring>
 
