@@ -233,12 +233,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         pdl_dependency_wait();
         if (quantise) {
             // -------------------------------------------------------- x to MXFP4
-            // unit = (stage, row); a warp's units are kWorkers apart
+            // A warp's units of each turn of the ring are (slot, row) pairs kWorkers apart, the same ones in every turn: so it
+            // has seen each of its slots' phases, and the parity that it waits for is never two phases away.
             const T *const x = static_cast<const T *>(p.x) + (int64_t)m0 * p.x_row_stride;
-            const int units = nkb * tokens;
             constexpr int kFlight = sizeof(T) == 4 ? 4 : 8;  // units whose loads a warp has in flight
-            auto fetch = [&](int u) {
-                const int i = u / tokens, r = u - i * tokens;
+            auto fetch = [&](int i, int r) {
                 const int64_t c = (int64_t)(kb0 + i) * kBK + lane * 8;
                 const T *const src = x + (int64_t)r * p.x_row_stride + c;
                 Vec8<T> raw{};
@@ -255,43 +254,41 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 return raw;
             };
-            // Rows written but not yet announced are units first .. last - 1 (in steps of kWorkers).
-            auto announce = [&](int first, int last) {
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0)
-                    for (int u = first; u < last; u += kWorkers) mbar_arrive(&xfull[u / tokens % S]);
-            };
-            for (int u0 = warp; ok && u0 < units; u0 += kFlight * kWorkers) {
-                Vec8<T> raw[kFlight];
+            for (int turn = 0; ok && turn * S < nkb; ++turn) {
+                const int units = min(S, nkb - turn * S) * tokens;
+                for (int u0 = warp; ok && u0 < units; u0 += kFlight * kWorkers) {
+                    Vec8<T> raw[kFlight];
 #pragma unroll
-                for (int j = 0; j < kFlight; ++j)
-                    if (u0 + j * kWorkers < units) raw[j] = fetch(u0 + j * kWorkers);
-                int first = u0;
-#pragma unroll
-                for (int j = 0; j < kFlight; ++j) {
-                    const int u = u0 + j * kWorkers;
-                    if (!ok || u >= units) break;
-                    const int i = u / tokens, r = u - i * tokens, s = i % S;
-                    if (i >= S) {  // the ring's stage is in use: what it waits for may need the rows above
-                        announce(first, u);
-                        first = u;
-                        ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((i / S) & 1) ^ 1, p.err, kErrTimeoutDequant));
-                        if (!ok) break;
+                    for (int j = 0; j < kFlight; ++j) {
+                        const int u = u0 + j * kWorkers, s = u / tokens;
+                        if (u < units) raw[j] = fetch(turn * S + s, u - s * tokens);
                     }
-                    float v[8];
-                    vec8_to_f32(raw[j], v);
-                    uint32_t codes;
-                    const uint32_t e = mx4_encode8(v, &codes);
-                    uint32_t word = e << (8 * ((lane >> 2) & 3));
-                    word |= __shfl_xor_sync(0xffffffffu, word, 4);
-                    word |= __shfl_xor_sync(0xffffffffu, word, 8);
-                    // 16-byte cells of a 128-byte row are swizzled by the row's place in eight
-                    *reinterpret_cast<uint32_t *>(smem + C::kBOff + s * C::kBBytes + r * kRowBytes + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = codes;
-                    if ((lane & 15) == 0)
-                        *reinterpret_cast<uint32_t *>(smem + C::kSfbOff + s * C::kSfBytes + (lane >> 4) * kSfTile + (r & 31) * 16 + (r >> 5) * 4) = word;
+#pragma unroll
+                    for (int j = 0; j < kFlight; ++j) {
+                        const int u = u0 + j * kWorkers, s = u / tokens, r = u - s * tokens;
+                        if (!ok || u >= units) break;
+                        if (turn > 0) {  // the MMAs of the turn before have read the slot
+                            ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], (turn & 1) ^ 1, p.err, kErrTimeoutDequant));
+                            if (!ok) break;
+                        }
+                        float v[8];
+                        vec8_to_f32(raw[j], v);
+                        uint32_t codes;
+                        const uint32_t e = mx4_encode8(v, &codes);
+                        uint32_t word = e << (8 * ((lane >> 2) & 3));
+                        word |= __shfl_xor_sync(0xffffffffu, word, 4);
+                        word |= __shfl_xor_sync(0xffffffffu, word, 8);
+                        // 16-byte cells of a 128-byte row are swizzled by the row's place in eight
+                        *reinterpret_cast<uint32_t *>(smem + C::kBOff + s * C::kBBytes + r * kRowBytes + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = codes;
+                        if ((lane & 15) == 0)
+                            *reinterpret_cast<uint32_t *>(smem + C::kSfbOff + s * C::kSfBytes + (lane >> 4) * kSfTile + (r & 31) * 16 + (r >> 5) * 4) = word;
+                    }
+                    // one fence for the batch, then its rows are announced
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (ok && lane == 0)
+                        for (int u = u0; u < min(u0 + kFlight * kWorkers, units); u += kWorkers) mbar_arrive(&xfull[u / tokens]);
                 }
-                if (ok) announce(first, min(u0 + kFlight * kWorkers, units));
             }
         }
         // ------------------------------------------------------------ epilogue

@@ -122,7 +122,7 @@ struct Heads {
 // A warp takes a token and a run of its q and k heads.  Needs dim % 8 == 0, with
 // halves pairs % 4 == 0, heads aligned as the layout says.  NORM: some weight is
 // given; POW2: dim / 8 is a power of two.
-template <typename T, Layout L, bool NORM, bool POW2>
+template <typename T, Layout L, bool NORM, bool POW2, int kTurns>
 __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qmm_rotary_args a, const int heads_per_warp) {
     constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;  // heads a lane group has in flight
     const int units = a.dim >> 3, at_a_time = 32 / units;
@@ -155,12 +155,25 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qm
             }
             if (!turned) {  // (while the first heads are on their way)
                 turned = true;
+                // Each lane turns pairs lane, lane + 32, ... and takes its four from the lanes that have them.
+                float c[kTurns], v[kTurns];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    cs[i] = twice(1.0f), sn[i] = twice(0.0f);
-                    if (live && pair + 2 * i < a.pairs) pair_turn(a, batch, token, pair + 2 * i, &cs[i].x, &sn[i].x);
-                    if (live && pair + 2 * i + 1 < a.pairs) pair_turn(a, batch, token, pair + 2 * i + 1, &cs[i].y, &sn[i].y);
+                for (int j = 0; j < kTurns; ++j) {
+                    c[j] = 1.0f, v[j] = 0.0f;
+                    if (lane + 32 * j < a.pairs) pair_turn(a, batch, token, lane + 32 * j, &c[j], &v[j]);
                 }
+                float mc[4], ms[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    mc[i] = 1.0f, ms[i] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < kTurns; ++j) {
+                        const float tc = __shfl_sync(0xffffffffu, c[j], (pair + i) & 31), ts = __shfl_sync(0xffffffffu, v[j], (pair + i) & 31);
+                        if ((pair + i) >> 5 == j) mc[i] = tc, ms[i] = ts;
+                    }
+                }
+                cs[0] = make_float2(mc[0], mc[1]), cs[1] = make_float2(mc[2], mc[3]);
+                sn[0] = make_float2(ms[0], ms[1]), sn[1] = make_float2(ms[2], ms[3]);
             }
             if (hb == h.h0) {
                 float2 we[2] = {twice(1.0f), twice(1.0f)}, wo[2] = {twice(1.0f), twice(1.0f)};
@@ -314,13 +327,16 @@ static qmm_status launch(const qmm_rotary_args &a, bool fast, bool wide, cudaStr
     if (grid.y > 65535) return fail(QMM_ERR_UNSUPPORTED, "rotary: %d heads are past the launch limits", heads);
     const bool norm = a.q_weight || a.k_weight, pow2 = (units & (units - 1)) == 0;
 #define QMM_ROTARY(L)                                                                            \
-    (!norm  ? rotary_kernel<T, L, false, true><<<grid, kWarps * 32, 0, st>>>(a, per)             \
-     : pow2 ? rotary_kernel<T, L, true, true><<<grid, kWarps * 32, 0, st>>>(a, per)              \
-            : rotary_kernel<T, L, true, false><<<grid, kWarps * 32, 0, st>>>(a, per))
+    (a.pairs <= 32 ? QMM_ROTARY_N(L, 1) : a.pairs <= 64 ? QMM_ROTARY_N(L, 2) : QMM_ROTARY_N(L, 4))
+#define QMM_ROTARY_N(L, N)                                                                       \
+    (!norm  ? rotary_kernel<T, L, false, true, N><<<grid, kWarps * 32, 0, st>>>(a, per)          \
+     : pow2 ? rotary_kernel<T, L, true, true, N><<<grid, kWarps * 32, 0, st>>>(a, per)           \
+            : rotary_kernel<T, L, true, false, N><<<grid, kWarps * 32, 0, st>>>(a, per))
     if (!fast) rotary_any_kernel<T><<<grid, kWarps * 32, 0, st>>>(a, per);
     else if (wide) QMM_ROTARY(kWide);
     else if (a.adjacent) QMM_ROTARY(kAdjacent);
     else QMM_ROTARY(kHalves);
+#undef QMM_ROTARY_N
 #undef QMM_ROTARY
     count_launch();
     const cudaError_t e = cudaGetLastError();

@@ -176,6 +176,17 @@ def test_product_at_odd_sizes(m, k, n):
     assert qib.device_error() == 0
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 12288, 9601), (3, 6400, 9728), (1, 20000, 9600), (2, 9000, 200), (17, 5000, 4800)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_deep_products_of_few_tokens(m, k, n, dtype):
+    # more stages than the ring holds, several times over, with and without a split of k
+    lin = layer(n, k, 1)
+    x = randn((m, k), 2, dtype=dtype).cuda()
+    y = lin.forward(x)
+    close(y, reference(lin, x))
+    assert torch.equal(y, lin.forward(qib.mx_quantize(x))) and qib.device_error() == 0
+
+
 @pytest.mark.parametrize("m,k,n", [(1, 512, 640), (9, 320, 96), (40, 1000, 1000), (513, 768, 2304), (2100, 512, 384)])
 @pytest.mark.parametrize("act,gated,residual,mul", [("gelu_tanh", False, False, False), ("none", True, True, False),
                                                     ("silu", False, True, True), ("gelu_tanh", True, True, True), (None, True, False, False)])
