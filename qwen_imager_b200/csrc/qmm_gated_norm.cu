@@ -25,33 +25,37 @@
 namespace qmm {
 namespace gnorm {
 
-// Eight elements of a 16-bit (BYTES 2) or 32-bit type at an aligned address, raw until used.
-template <int BYTES>
-struct Raw8 {
-    uint4 w[BYTES / 2];
+// Eight elements of a 16-bit (BYTES 2) or 32-bit type, raw until used: at a 16-byte
+// aligned address (VEC), or the aligned 16-byte pieces that hold them.
+template <int BYTES, bool VEC>
+struct Held {
+    static constexpr int kBytes = BYTES, kPieces = BYTES / 2 + (VEC ? 0 : 1);
+    uint4 piece[kPieces];
 };
+template <int BYTES>
+using Raw8 = Held<BYTES, true>;
 template <int BYTES>
 __device__ __forceinline__ Raw8<BYTES> load_raw8(const void *p, int64_t index) {
     Raw8<BYTES> r;
     const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(p) + index * BYTES);
 #pragma unroll
-    for (int i = 0; i < BYTES / 2; ++i) r.w[i] = q[i];
+    for (int i = 0; i < BYTES / 2; ++i) r.piece[i] = q[i];
     return r;
 }
 template <int BYTES>
 __device__ __forceinline__ void raw8_to_f32(const Raw8<BYTES> &r, bool f16, float (&v)[8]) {
     if constexpr (BYTES == 4) {
         Vec8<float> t;
-        t.w[0] = r.w[0];
-        t.w[1] = r.w[1];
+        t.w[0] = r.piece[0];
+        t.w[1] = r.piece[1];
         vec8_to_f32(t, v);
     } else if (f16) {
         Vec8<F16> t;
-        t.w[0] = r.w[0];
+        t.w[0] = r.piece[0];
         vec8_to_f32(t, v);
     } else {
         Vec8<Bf16> t;
-        t.w[0] = r.w[0];
+        t.w[0] = r.piece[0];
         vec8_to_f32(t, v);
     }
 }
@@ -136,15 +140,88 @@ __device__ __forceinline__ void encode_lane(const qmm_gated_norm_args &a, int64_
     if (lane == 0 && b < tiles * 4) a.n_scales[mx4_scale_offset(row, b, tiles)] = (uint8_t)e;
 }
 
-// Eight elements of one thread's row: as vectors (VEC) or one by one.
-template <typename T, int BYTES, bool VEC>
-struct Held {
-    Raw8<BYTES> v;
-};
-template <typename T, int BYTES>
-struct Held<T, BYTES, false> {
-    uint32_t e[8];  // bits of each element
-};
+// w[0 .. N) = the words `bytes` (0 .. 15, the same in the whole warp) behind w[0].
+template <int N, bool HALVES>
+__device__ __forceinline__ void shift_words(uint32_t (&w)[N + 4], uint32_t bytes) {
+    const bool two = bytes & 8, one = bytes & 4;
+#pragma unroll
+    for (int k = 0; k < N + 2; ++k) w[k] = two ? w[k + 2] : w[k];
+#pragma unroll
+    for (int k = 0; k < N + 1; ++k) w[k] = one ? w[k + 1] : w[k];
+    if constexpr (HALVES) {
+        const uint32_t s = (bytes & 2) * 8;
+#pragma unroll
+        for (int k = 0; k < N; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], s);
+    }
+}
+
+// The row of `hidden` elements at p by the 16-byte pieces that hold it: columns [c(i),
+// c(i) + 8), c(i) = first + i * step.  Its first and last piece reach into the rows
+// beside it; they are not read where that would be outside [base, end), the operand.
+template <int BYTES, int VPT>
+__device__ __forceinline__ void fetch_pieces(Held<BYTES, false> (&held)[VPT], uintptr_t p, int first, int step, int hidden, uintptr_t base, uintptr_t end) {
+    constexpr int kPieces = Held<BYTES, false>::kPieces;
+    const uintptr_t a = p & ~(uintptr_t)15, past = p + (int64_t)hidden * BYTES;
+    if (a >= base && ((past + 15) & ~(uintptr_t)15) <= end) {
+        const int last = (int)(past - 1 - a) & ~15;  // lanes past the row read its last piece
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k)
+                held[i].piece[k] = *reinterpret_cast<const uint4 *>(a + min((first + i * step) * BYTES + 16 * k, last));
+    } else {  // the pieces at the operand's ends: one element at a time
+#pragma unroll
+        for (int i = 0; i < VPT; ++i)
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) {
+                const uintptr_t q = a + (int64_t)(first + i * step) * BYTES + 16 * k;
+                held[i].piece[k] = make_uint4(0, 0, 0, 0);
+                if (q >= base && q + 16 <= end) {
+                    held[i].piece[k] = *reinterpret_cast<const uint4 *>(q);
+                } else if (q < past) {
+                    uint32_t w[4] = {};
+#pragma unroll
+                    for (int e = 0; e < 16 / BYTES; ++e) {
+                        const uintptr_t at = q + e * BYTES;
+                        if (at >= p && at < past) {
+                            if constexpr (BYTES == 4) w[e] = *reinterpret_cast<const uint32_t *>(at);
+                            else w[e / 2] |= (uint32_t)*reinterpret_cast<const uint16_t *>(at) << (16 * (e & 1));
+                        }
+                    }
+                    held[i].piece[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+    }
+}
+
+// A warp's eight columns a lane, `count` in all, to any element-aligned address: through
+// shared memory the lanes take each other's parts of the aligned 16-byte pieces, and the
+// elements before the first (`skip` bytes) and after the last piece go one by one.
+template <typename T>
+__device__ __forceinline__ void store_shifted(T *to, uint32_t skip, int count, const float (&v)[8], uint4 *stage) {
+    constexpr int kWords = sizeof(T) * 2, kPieces = kWords / 4, kEach = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31;
+    uint32_t w[kWords + 4];
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+        if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(v[k]);
+        else w[k] = pack2<T>(v[2 * k], v[2 * k + 1]);
+    }
+    __syncwarp();  // the stage's last readers are through
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k) stage[lane * kPieces + k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    __syncwarp();
+    const uint4 next = stage[min(lane + 1, 31) * kPieces];  // (lane 31 has whole pieces only where nothing is shifted)
+    w[kWords] = next.x, w[kWords + 1] = next.y, w[kWords + 2] = next.z, w[kWords + 3] = next.w;
+    const int head = min((int)(skip / sizeof(T)), count), body = (count - head) / kEach;
+    shift_words<kWords, sizeof(T) == 2>(w, skip);
+    uint4 *const pieces = reinterpret_cast<uint4 *>(reinterpret_cast<uintptr_t>(to) + skip);
+#pragma unroll
+    for (int k = 0; k < kPieces; ++k)
+        if (lane * kPieces + k < body) pieces[lane * kPieces + k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    const int at = lane < kEach ? lane : head + (body - 1) * kEach + lane;
+    if (lane < kEach ? lane < head : lane < 2 * kEach && at < count) to[at] = reinterpret_cast<const T *>(stage)[at];
+}
 
 // blockDim.x threads a row, blockDim.y rows side by side (more than one only with 32
 // threads a row).  VEC: x and branch rows, and outputs, 16-byte aligned, hidden a
@@ -154,68 +231,82 @@ __global__ void __launch_bounds__(MAXT, MINB)
     gated_norm_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group, const uint32_t rows_each, const bool vec_aligned) {
     extern __shared__ float4 shared_vectors[];  // A, S, H of each row side by side: threads * VPT * 8 columns (0 past the row), every thread's its own
     __shared__ __align__(16) float red[4][MAXT / 32];
+    __shared__ uint4 stage[VEC ? 1 : MAXT / 32][VEC ? 1 : 16 * sizeof(T)];  // a warp's own
     RowSum<MAXT / 32> row_sum{red};
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
     const int hidden = (int)a.hidden;
     const float inv_hidden = 1.0f / (float)hidden;
-    auto column = [&](int i, int q) { return VEC ? (i * threads + tid) * 8 + q : (i * 8 + q) * threads + tid; };
-    auto valid = [&](int i, int q) { return column(i, VEC ? 0 : q) < hidden; };
-    constexpr int XB = (int)sizeof(T);
+    auto column = [&](int i) { return (i * threads + tid) * 8; };
     const bool f16_branch = a.branch_elem == QMM_ELEM_F16;
     const int span = threads * VPT * 2;  // float4 a vector
     float4 *const vectors = shared_vectors + threadIdx.y * 3 * span;
 
-    Held<T, XB, VEC> rx[VPT];
-    Held<T, BBYTES, VEC> rb[VPT];
+    constexpr int XB = (int)sizeof(T);
+    Held<XB, VEC> rx[VPT];
+    Held<BBYTES, VEC> rb[VPT] = {};
+    auto row_at = [](const void *p, int64_t row, int64_t stride, int bytes) { return reinterpret_cast<uintptr_t>(p) + row * stride * bytes; };
     auto fetch = [&](int64_t row) {
+        if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            rx[i] = {};
-            rb[i] = {};
-            if constexpr (VEC) {
-                if (valid(i, 0)) {
-                    rx[i].v = load_raw8<XB>(a.x, row * a.x_stride + column(i, 0));
-                    if (a.branch) rb[i].v = load_raw8<BBYTES>(a.branch, row * a.branch_stride + column(i, 0));
+            for (int i = 0; i < VPT; ++i) {
+                rx[i] = {};
+                rb[i] = {};
+                if (column(i) < hidden) {
+                    rx[i] = load_raw8<XB>(a.x, row * a.x_stride + column(i));
+                    if (a.branch) rb[i] = load_raw8<BBYTES>(a.branch, row * a.branch_stride + column(i));
                 }
-            } else {
+            }
+        } else {
+            auto pieces = [&](auto &held, const void *p, int64_t stride, int bytes) {
+                const uintptr_t base = reinterpret_cast<uintptr_t>(p);
+                fetch_pieces(held, row_at(p, row, stride, bytes), tid * 8, threads * 8, hidden, base, row_at(p, a.rows - 1, stride, bytes) + (int64_t)hidden * bytes);
+            };
+            pieces(rx, a.x, a.x_stride, XB);
+            if (a.branch) pieces(rb, a.branch, a.branch_stride, BBYTES);
+        }
+    };
+    // Zeroes columns past the row, which a whole vector seldom has.
+    auto clear = [&](int i, float2 (&v)[4]) {
+        const int left = hidden - column(i);
+        if (VEC || left < 8)
+        {
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    if (valid(i, q)) {
-                        const int64_t c = column(i, q);
-                        rx[i].e[q] = XB == 4 ? static_cast<const uint32_t *>(a.x)[row * a.x_stride + c] : static_cast<const uint16_t *>(a.x)[row * a.x_stride + c];
-                        if (a.branch)
-                            rb[i].e[q] = BBYTES == 4 ? static_cast<const uint32_t *>(a.branch)[row * a.branch_stride + c]
-                                                     : static_cast<const uint16_t *>(a.branch)[row * a.branch_stride + c];
-                    }
-                }
+            for (int q = 0; q < 4; ++q) {
+                v[q].x = (VEC ? 0 : 2 * q) >= left ? 0.0f : v[q].x;
+                v[q].y = (VEC ? 0 : 2 * q + 1) >= left ? 0.0f : v[q].y;
             }
         }
     };
-    auto unpack = [&](const auto &held, bool f16, float2 (&v)[4]) {
-        constexpr bool kWide = std::is_same<decltype(held), const Held<T, 4, VEC> &>::value;
-        float w[8];
-        (void)kWide;
-        if constexpr (VEC) {
-            raw8_to_f32(held.v, f16, w);
+    auto unpack = [&](const auto &held, int i, uint32_t offset, bool f16, float2 (&v)[4]) {
+        constexpr int BYTES = std::decay_t<decltype(held)>::kBytes, kPieces = std::decay_t<decltype(held)>::kPieces, kWords = BYTES * 2;
+        uint32_t w[kWords + 4];
+#pragma unroll
+        for (int k = 0; k < kPieces; ++k) w[4 * k] = held.piece[k].x, w[4 * k + 1] = held.piece[k].y, w[4 * k + 2] = held.piece[k].z, w[4 * k + 3] = held.piece[k].w;
+        if constexpr (!VEC) shift_words<kWords, BYTES == 2>(w, offset);
+        if constexpr (BYTES == 4) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = make_float2(__uint_as_float(w[2 * q]), __uint_as_float(w[2 * q + 1]));
+        } else if (f16) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = unpack2<F16>(w[q]);
         } else {
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-                w[q] = kWide ? __uint_as_float(held.e[q]) : f16 ? elem_to_f32(F16{(uint16_t)held.e[q]}) : elem_to_f32(Bf16{(uint16_t)held.e[q]});
+            for (int q = 0; q < 4; ++q) v[q] = unpack2<Bf16>(w[q]);
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = make_float2(w[2 * q], w[2 * q + 1]);
+        if constexpr (!VEC) clear(i, v);
     };
     auto store = [&](void *p, int64_t base, const float2 (&v)[VPT][4]) {
         T *const o = static_cast<T *>(p) + base;
+        [[maybe_unused]] const uint32_t skip = -(uint32_t)reinterpret_cast<uintptr_t>(o) & 15u;  // (a warp's columns begin at multiples of 256)
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             const float w[8] = {v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y, v[i][2].x, v[i][2].y, v[i][3].x, v[i][3].y};
+            const int c = column(i);
             if constexpr (VEC) {
-                if (valid(i, 0)) store_vec8(o + column(i, 0), w);
+                if (c < hidden) store_vec8(o + c, w);
             } else {
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (valid(i, q)) o[column(i, q)] = elem_from_f32<T>(w[q]);
+                const int from = c - lane * 8;  // the warp's first column
+                if (from < hidden) store_shifted(o + from, skip, min(256, hidden - from), w, stage[threadIdx.y + (tid >> 5)]);
             }
         }
     };
@@ -236,20 +327,20 @@ __global__ void __launch_bounds__(MAXT, MINB)
                 o[0] = make_float4(f[0], f[1], f[2], f[3]);
                 o[threads] = make_float4(f[4], f[5], f[6], f[7]);
             };
-            if (VEC && vec_aligned) {  // every load is on its way before the first is used
-                const bool in = valid(i, 0);
-                const int c = column(i, 0);
+            if (vec_aligned && (VEC || column(i) + 8 <= hidden)) {  // every load is on its way before the first is used
+                const int c = column(i);
+                const bool in = c < hidden;
                 auto raw = [&](const void *p, int64_t at) {
                     Raw8<4> r{};
                     if (in && p) {
                         if (a.vec_elem == QMM_ELEM_F32) r = load_raw8<4>(p, at + c);
-                        else r.w[0] = load_raw8<2>(p, at + c).w[0];
+                        else r.piece[0] = load_raw8<2>(p, at + c).piece[0];
                     }
                     return r;
                 };
                 auto values = [&](const Raw8<4> &r, const void *p, float none, float (&w)[8]) {
                     if (a.vec_elem == QMM_ELEM_F32) raw8_to_f32(r, false, w);
-                    else raw8_to_f32(Raw8<2>{{r.w[0]}}, a.vec_elem == QMM_ELEM_F16, w);
+                    else raw8_to_f32(Raw8<2>{{r.piece[0]}}, a.vec_elem == QMM_ELEM_F16, w);
                     if (!p) {
 #pragma unroll
                         for (int q = 0; q < 8; ++q) w[q] = none;
@@ -271,20 +362,34 @@ __global__ void __launch_bounds__(MAXT, MINB)
                 values(r4, a.shift, 0.0f, f);
                 put(2, f);
             } else {
-                float f[3][8];
+                // One element at a time, the loads of four columns on their way together.
+                auto value = [&](uint32_t w) {
+                    return a.vec_elem == QMM_ELEM_F32 ? __uint_as_float(w) : a.vec_elem == QMM_ELEM_F16 ? elem_to_f32(F16{(uint16_t)w}) : elem_to_f32(Bf16{(uint16_t)w});
+                };
+#pragma unroll(VEC ? 1 : 2)
+                for (int half = 0; half < 2; ++half) {
+                    const int c = column(i) + 4 * half;
+                    auto raw = [&](const void *p, int64_t at, uint32_t (&w)[4]) {
+                        const int n = p ? hidden - c : 0;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    f[0][q] = f[1][q] = f[2][q] = 0.0f;
-                    if (valid(i, q)) {
-                        const int64_t c = column(i, q);
-                        f[0][q] = (a.post_weight ? load_elem(a.post_weight, a.vec_elem, c) : 1.0f) * (a.gate ? load_elem(a.gate, a.vec_elem, gate + c) : 1.0f);
-                        const float w = a.pre_weight ? load_elem(a.pre_weight, a.vec_elem, c) : 1.0f;
-                        f[1][q] = a.scale ? fmaf(w, load_elem(a.scale, a.vec_elem, scale + c), w) : w;
-                        if (a.shift) f[2][q] = load_elem(a.shift, a.vec_elem, shift + c);
+                        for (int q = 0; q < 4; ++q) {
+                            w[q] = 0;
+                            if (q < n) w[q] = a.vec_elem == QMM_ELEM_F32 ? static_cast<const uint32_t *>(p)[at + c + q] : static_cast<const uint16_t *>(p)[at + c + q];
+                        }
+                    };
+                    uint32_t r[5][4];
+                    raw(a.post_weight, 0, r[0]), raw(a.gate, gate, r[1]), raw(a.pre_weight, 0, r[2]), raw(a.scale, scale, r[3]), raw(a.shift, shift, r[4]);
+                    float f[3][4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float one = c + q < hidden ? 1.0f : 0.0f, w = a.pre_weight ? value(r[2][q]) : one;
+                        f[0][q] = (a.post_weight ? value(r[0][q]) : one) * (a.gate ? value(r[1][q]) : 1.0f);
+                        f[1][q] = fmaf(w, value(r[3][q]), w);
+                        f[2][q] = value(r[4][q]);
                     }
-                }
 #pragma unroll
-                for (int k = 0; k < 3; ++k) put(k, f[k]);
+                    for (int k = 0; k < 3; ++k) mine(k, i)[half * threads] = make_float4(f[k][0], f[k][1], f[k][2], f[k][3]);
+                }
             }
         }
     };
@@ -299,8 +404,11 @@ __global__ void __launch_bounds__(MAXT, MINB)
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                v[i][q] = add_f32x2(v[i][q], make_float2(valid(i, 2 * q) ? -mean : 0.0f, valid(i, 2 * q + 1) ? -mean : 0.0f));
+            for (int q = 0; q < 4; ++q) v[i][q] = add_f32x2(v[i][q], twice(VEC && column(i) >= hidden ? 0.0f : -mean));
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int i = 0; i < VPT; ++i) clear(i, v[i]);
+        }
     };
     auto rms = [&](const float2 (&v)[VPT][4]) {
         float2 s = twice(0.0f);
@@ -315,17 +423,18 @@ __global__ void __launch_bounds__(MAXT, MINB)
     pdl_launch_dependents();  // a product behind this pass sets itself up meanwhile; it waits for the grid before it reads
     const uint32_t first = (blockIdx.x * blockDim.y + threadIdx.y) * rows_each, last = min(first + rows_each, (uint32_t)a.rows);
     if (first < last) fetch(first);
-    uint32_t group = UINT32_MAX;
+    uint32_t group_end = first;
     for (uint32_t row = first; row < last; ++row) {
-        if (row / rows_per_group != group) {
-            group = row / rows_per_group;
+        if (row == group_end) {
+            const uint32_t group = row / rows_per_group;
+            group_end = (group + 1) * rows_per_group;
             take_vectors(group);
         }
         float2 x[VPT][4], h[VPT][4];
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
-            unpack(rx[i], std::is_same<T, F16>::value, x[i]);
-            unpack(rb[i], f16_branch, h[i]);
+            unpack(rx[i], i, VEC ? 0u : (uint32_t)row_at(a.x, row, a.x_stride, XB) & 15u, std::is_same<T, F16>::value, x[i]);
+            unpack(rb[i], i, VEC ? 0u : (uint32_t)row_at(a.branch, row, a.branch_stride, BBYTES) & 15u, f16_branch, h[i]);
         }
         if (row + 1 < last) fetch((int64_t)row + 1);
         const float2 c2 = twice(a.residual_scale);
@@ -364,27 +473,17 @@ __global__ void __launch_bounds__(MAXT, MINB)
         // MXFP4: columns past the row are zeros of its last block.
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
+            clear(i, x[i]);  // (0 times an infinite or NaN statistic)
             float w[8] = {x[i][0].x, x[i][0].y, x[i][1].x, x[i][1].y, x[i][2].x, x[i][2].y, x[i][3].x, x[i][3].y};
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-                if (!valid(i, q)) w[q] = 0.0f;  // (0 times an infinite or NaN statistic)
-            if constexpr (VEC) {
-                const int c = column(i, 0);
-                uint32_t codes;
-                const uint32_t e = mx4_encode8(w, &codes);
-                if (c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = codes;
-                uint32_t word = e << (8 * ((lane >> 2) & 3));
-                word |= __shfl_xor_sync(0xffffffffu, word, 4);
-                word |= __shfl_xor_sync(0xffffffffu, word, 8);
-                const int64_t b = c / kMxBlock;
-                if ((lane & 15) == 0 && b < tiles * 4) *reinterpret_cast<uint32_t *>(a.n_scales + mx4_scale_offset(row, b, tiles)) = word;
-            } else {
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    if (column(i, q) - lane >= tiles * 128) continue;  // the same in the whole warp
-                    encode_lane(a, row, column(i, q), w[q], pitch, tiles);
-                }
-            }
+            const int c = column(i);
+            uint32_t codes;
+            const uint32_t e = mx4_encode8(w, &codes);
+            if (c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = codes;
+            uint32_t word = e << (8 * ((lane >> 2) & 3));
+            word |= __shfl_xor_sync(0xffffffffu, word, 4);
+            word |= __shfl_xor_sync(0xffffffffu, word, 8);
+            const int64_t b = c / kMxBlock;
+            if ((lane & 15) == 0 && b < tiles * 4) *reinterpret_cast<uint32_t *>(a.n_scales + mx4_scale_offset(row, b, tiles)) = word;
         }
     }
 }

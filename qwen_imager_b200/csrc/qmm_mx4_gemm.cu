@@ -78,7 +78,6 @@ struct Params {
     int32_t nkb, sf_tiles;       // stages along k; scale tiles along k
     int32_t m_tiles, n_tiles;
     int32_t b_row_tiles;         // 128-row scale tiles of W
-    int32_t tma_out;             // y (and the residual) by TMA: rows on 16-byte boundaries
     uint32_t *err;
 };
 
@@ -103,10 +102,108 @@ __device__ __forceinline__ void request_residual(const CUtensorMap *tmap_res, co
     }
 }
 
+// 32 tokens x 32 features in a warp's staging buffer, and their rows in global memory
+// off 16-byte boundaries, which move by aligned 4-byte words, half a warp a token.
+// Where a token's first feature is the upper half of a word (odd), its cells hold the
+// words one feature earlier, and the last word is the lane's own (`behind`).  A lane's
+// tokens are two apart, so the words it moves are of odd tokens or of none.
+struct WordRows {
+    uint8_t *stage;
+    int64_t own;         // element of token `lane`
+    int64_t first;       // element in the lower half of the lane's first word
+    int nf, nt, f;       // features and tokens here; the feature of `first`
+    __device__ __forceinline__ WordRows(const Params &p, uint8_t *buffer, int f0, int m0) : stage(buffer) {
+        const int lane = threadIdx.x & 31, side = lane >> 4;
+        nf = min(kChunk, p.n - f0), nt = min(32, p.m - m0);
+        own = (int64_t)(m0 + lane) * p.n + f0;
+        const int64_t e = (int64_t)(m0 + side) * p.n + f0;
+        f = 2 * (lane & 15) - (int)(e & 1);
+        first = e + f;
+    }
+    __device__ __forceinline__ bool odd() const { return own & 1; }
+    __device__ __forceinline__ uint4 *cell(int g) const {
+        const int lane = threadIdx.x & 31;
+        return reinterpret_cast<uint4 *>(stage + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4));
+    }
+    // The lane's word of token t0 + 2 u + lane / 16, t0 a multiple of 8.
+    __device__ __forceinline__ uint32_t *word(int t0, int u) const {
+        const int lane = threadIdx.x & 31;
+        return reinterpret_cast<uint32_t *>(stage + (t0 + 2 * u + (lane >> 4)) * 64 + ((((lane & 15) >> 2) ^ (u & 3)) << 4) + (lane & 3) * 4);
+    }
+    __device__ __forceinline__ void load(const uint16_t *p, int n) const {
+        const int lane = threadIdx.x & 31;
+        uint32_t behind = 0;
+        if (odd() && lane < nt && nf == kChunk) behind = p[own + kChunk - 1];
+        const uint16_t *from = p + first;
+        const int tokens = f < nf ? nt - (lane >> 4) : 0;
+#pragma unroll 1
+        for (int t0 = 0; t0 < 32; t0 += 16) {
+            uint32_t w[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                w[u] = 0;
+                if (t0 + 2 * u < tokens) {  // (before the first feature: the token before's last; past the last: not read)
+                    if (f + 1 < nf) w[u] = *reinterpret_cast<const uint32_t *>(from);
+                    else w[u] = *from;
+                }
+                from += 2 * (int64_t)n;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) *word(t0, u) = w[u];
+        }
+        __syncwarp();
+        if (odd()) {
+            uint4 c[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) c[g] = *cell(g);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *cell(g) = make_uint4(__funnelshift_r(c[g].x, c[g].y, 16), __funnelshift_r(c[g].y, c[g].z, 16), __funnelshift_r(c[g].z, c[g].w, 16),
+                                      __funnelshift_r(c[g].w, g < 3 ? c[(g + 1) & 3].x : behind, 16));
+        }
+    }
+    // w: the lane's token.
+    __device__ __forceinline__ void store(uint16_t *y, int n, uint32_t (&w)[16]) const {
+        const int lane = threadIdx.x & 31;
+        const uint32_t behind = w[15] >> 16;
+        if (odd()) {
+#pragma unroll
+            for (int i = 15; i >= 0; --i) w[i] = __funnelshift_l(i ? w[i > 0 ? i - 1 : 0] : 0u, w[i], 16);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) *cell(g) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
+        if (lane < nt) {  // a token's first and last feature, where they are half a word
+            if (odd()) y[own] = (uint16_t)(w[0] >> 16);
+            if ((nf + odd()) & 1) {
+                const int last = (nf - 1 + odd()) >> 1;
+                const uint32_t *const c = reinterpret_cast<const uint32_t *>(cell((last & 15) >> 2)) + (last & 3);
+                y[own + nf - 1] = (uint16_t)(last < 16 ? *c : behind);
+            }
+        }
+        __syncwarp();
+        uint16_t *to = y + first;
+        const int tokens = f >= 0 && f + 1 < nf ? nt - (lane >> 4) : 0;
+#pragma unroll 1
+        for (int t0 = 0; t0 < 32; t0 += 8) {
+            uint32_t c[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) c[u] = *word(t0, u);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (t0 + 2 * u < tokens) *reinterpret_cast<uint32_t *>(to) = c[u];
+                to += 2 * (int64_t)n;
+            }
+        }
+        __syncwarp();
+    }
+};
+
 // One warp's 32 tokens x 32 features, from the accumulators in r (a token a lane)
-// through its staging buffer to y.
+// through its staging buffer to y.  TMA: rows of y and the residual lie on 16-byte
+// boundaries and move by TMA; the residual is in the buffer already.
+template <bool TMA>
 __device__ __forceinline__ void chunk_finish(const Params &p, const CUtensorMap *tmap_y, const ChunkOut &o, const float *vec, uint32_t (&r)[32],
-                                             int f0, int m0, bool res_tma) {
+                                             int f0, int m0) {
     const int lane = threadIdx.x & 31;
     const float4 *const bias = reinterpret_cast<const float4 *>(vec), *const gate = bias + kChunk / 4;
     // Each step over all 32 features: its branch is taken once, and the exponentials overlap.
@@ -143,20 +240,9 @@ __device__ __forceinline__ void chunk_finish(const Params &p, const CUtensorMap 
         }
     }
     auto cell = [&](int g) { return reinterpret_cast<uint4 *>(o.stage + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)); };
-    // This lane's feature of token t, where rows of y are not on 16-byte boundaries and a warp moves them one by one.
-    auto element = [&](int t) { return reinterpret_cast<uint16_t *>(o.stage + t * 64 + (((lane >> 3) ^ ((t >> 1) & 3)) << 4) + (lane & 7) * 2); };
-    const int rows = f0 + lane < p.n ? min(32, p.m - m0) : 0;
-    const int64_t at = (int64_t)m0 * p.n + f0 + lane;
-    if (p.ep.residual && !res_tma) {
-#pragma unroll 1
-        for (int t0 = 0; t0 < 32; t0 += 4) {
-            uint16_t w[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) w[t] = t0 + t < rows ? p.ep.residual[at + (int64_t)(t0 + t) * p.n] : 0;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) *element(t0 + t) = w[t];
-        }
-        __syncwarp();
+    [[maybe_unused]] const WordRows rows(p, o.stage, f0, m0);
+    if constexpr (!TMA) {
+        if (p.ep.residual) rows.load(p.ep.residual, p.n);
     }
     if (p.ep.residual) {
 #pragma unroll
@@ -169,15 +255,16 @@ __device__ __forceinline__ void chunk_finish(const Params &p, const CUtensorMap 
             for (int e = 0; e < 8; ++e) v[g * 8 + e] = p.ep.res_mul ? res[e] * v[g * 8 + e] : res[e] + v[g * 8 + e];
         }
     }
-    if (p.tma_out && !res_tma) {
-        if (lane == 0) bulk_wait_read<0>();  // the last store has left the buffer
-        __syncwarp();
-    }
+    uint32_t w[16];
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-        *cell(g) = make_uint4(pack_bf16x2_rn(v[8 * g], v[8 * g + 1]), pack_bf16x2_rn(v[8 * g + 2], v[8 * g + 3]),
-                              pack_bf16x2_rn(v[8 * g + 4], v[8 * g + 5]), pack_bf16x2_rn(v[8 * g + 6], v[8 * g + 7]));
-    if (p.tma_out) {
+    for (int i = 0; i < 16; ++i) w[i] = pack_bf16x2_rn(v[2 * i], v[2 * i + 1]);
+    if constexpr (TMA) {
+        if (!p.ep.residual) {
+            if (lane == 0) bulk_wait_read<0>();  // the last store has left the buffer
+            __syncwarp();
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) *cell(g) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -185,28 +272,18 @@ __device__ __forceinline__ void chunk_finish(const Params &p, const CUtensorMap 
             bulk_commit();
         }
     } else {
-        __syncwarp();
-#pragma unroll 1
-        for (int t0 = 0; t0 < 32; t0 += 4) {
-            uint16_t w[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) w[t] = *element(t0 + t);
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (t0 + t < rows) p.y[at + (int64_t)(t0 + t) * p.n] = w[t];
-        }
-        __syncwarp();
+        rows.store(p.y, p.n, w);
     }
 }
 
 // A tile's chunks of one warp.  feature(c): the c-th chunk's first feature (p.n or more: none); column(c): its accumulator
 // column; loaded(c) runs once chunk c is in registers; q counts the warp's chunks so far.  False: a wait ran out.
-template <bool CLUSTER, typename Feature, typename Column, typename Loaded>
+template <bool CLUSTER, bool TMA, typename Feature, typename Column, typename Loaded>
 __device__ __forceinline__ bool tile_epilogue(const Params &p, const CUtensorMap *tmap_y, const CUtensorMap *tmap_res, const ChunkOut &o, uint64_t *acc_full,
                                               uint32_t parity, uint32_t tmem, int m0, uint32_t &q, const Feature &feature, const Column &column,
                                               const Loaded &loaded) {
     const int lane = threadIdx.x & 31;
-    const bool res_tma = p.tma_out && p.ep.residual;
+    const bool res_tma = TMA && p.ep.residual;
     // A quadrant past the last token or a chunk past the last feature has nothing to store.
     auto live = [&](int c) { return m0 < p.m && feature(c) < p.n; };
     bool requested = res_tma && live(0);
@@ -239,7 +316,7 @@ __device__ __forceinline__ bool tile_epilogue(const Params &p, const CUtensorMap
         loaded(c);
         if (live(c)) {
             if (res_tma && !__all_sync(0xffffffffu, mbar_wait(o.res_full, q & 1, p.err, kErrTimeoutEpilogue))) return false;
-            chunk_finish(p, tmap_y, o, o.vec + c * 2 * kChunk, r, feature(c), m0, res_tma);
+            chunk_finish<TMA>(p, tmap_y, o, o.vec + c * 2 * kChunk, r, feature(c), m0);
             requested = false;
             ++q;
         }
@@ -247,7 +324,7 @@ __device__ __forceinline__ bool tile_epilogue(const Params &p, const CUtensorMap
     return true;
 }
 
-template <int TN>
+template <int TN, bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
     mx4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                     const __grid_constant__ CUtensorMap tmap_y, const __grid_constant__ CUtensorMap tmap_res, const Params p) {
@@ -284,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kProducer && lane == 0) {
         tma_prefetch_desc(&tmap_a);
         tma_prefetch_desc(&tmap_b);
-        if (p.tma_out) tma_prefetch_desc(&tmap_y);
-        if (p.tma_out && p.ep.residual) tma_prefetch_desc(&tmap_res);
+        if (TMA) tma_prefetch_desc(&tmap_y);
+        if (TMA && p.ep.residual) tma_prefetch_desc(&tmap_res);
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -405,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&acc_empty[b]);
             };
-            if (!tile_epilogue<false>(p, &tmap_y, &tmap_res, o, &acc_full[b], (lt >> 1) & 1, tmem, m0, q, feature, column, loaded)) break;
+            if (!tile_epilogue<false, TMA>(p, &tmap_y, &tmap_res, o, &acc_full[b], (lt >> 1) & 1, tmem, m0, q, feature, column, loaded)) break;
         }
         if (lane == 0) bulk_wait_all();
     }
@@ -480,6 +557,7 @@ __device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *m
         : "memory");
 }
 
+template <bool TMA>
 __global__ void __launch_bounds__(kThreads, 1)
     mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb,
@@ -524,8 +602,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_prefetch_desc(&tmap_b);
         tma_prefetch_desc(&tmap_sfa);
         tma_prefetch_desc(&tmap_sfb);
-        if (p.tma_out) tma_prefetch_desc(&tmap_y);
-        if (p.tma_out && p.ep.residual) tma_prefetch_desc(&tmap_res);
+        if (TMA) tma_prefetch_desc(&tmap_y);
+        if (TMA && p.ep.residual) tma_prefetch_desc(&tmap_res);
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -643,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(c == 0 ? shared_cols : &acc_empty[b]), 0));
             };
-            if (!tile_epilogue<true>(p, &tmap_y, &tmap_res, o, &acc_full[b], (lt >> 1) & 1, tmem, m0, q, feature, column, loaded)) break;
+            if (!tile_epilogue<true, TMA>(p, &tmap_y, &tmap_res, o, &acc_full[b], (lt >> 1) & 1, tmem, m0, q, feature, column, loaded)) break;
         }
         if (lane == 0) bulk_wait_all();
     }
@@ -655,6 +733,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_dealloc_pair(tmem, 512);
     }
 }
+
+// Rows of y and the residual on 16-byte boundaries.
+static bool by_tma(int64_t n) { return n % 8 == 0; }
 
 // Scales as [row tiles][256-byte rows]: a stage's two tiles of a row tile are four consecutive rows.
 static qmm_status map_scales(CUtensorMap *map, const uint8_t *scales, int64_t rows, int64_t k, uint32_t row_tiles_a_box) {
@@ -683,9 +764,8 @@ static qmm_status make_problem(Problem &q, const qmm_mx4 &w, const qmm_mx4 &x, c
     if (s != QMM_OK) return s;
     s = map_2d(&q.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, w.codes, pitch, (uint64_t)w.rows, pitch, kRowBytes, (uint32_t)b_rows, CU_TENSOR_MAP_SWIZZLE_128B);
     if (s != QMM_OK) return s;
-    const bool tma_out = w.rows % 8 == 0;  // rows of y on 16-byte boundaries
     q.y = q.res = q.a;
-    if (tma_out) {
+    if (by_tma(w.rows)) {
         s = map_2d(&q.y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, y, (uint64_t)w.rows, (uint64_t)x.rows, (uint64_t)w.rows * 2, kChunk, 32, CU_TENSOR_MAP_SWIZZLE_64B);
         if (s == QMM_OK && ep.residual)
             s = map_2d(&q.res, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ep.residual, (uint64_t)w.rows, (uint64_t)x.rows, (uint64_t)w.rows * 2, kChunk, 32,
@@ -706,16 +786,15 @@ static qmm_status make_problem(Problem &q, const qmm_mx4 &w, const qmm_mx4 &x, c
     p.m_tiles = (int32_t)mt;
     p.n_tiles = (int32_t)nt;
     p.b_row_tiles = (int32_t)mx4_row_tiles(w.rows);
-    p.tma_out = tma_out ? 1 : 0;
     p.err = device_error_word();
     return QMM_OK;
 }
 
-template <int TN>
+template <int TN, bool TMA>
 static qmm_status launch_gemm(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epilogue &ep, uint16_t *y, cudaStream_t st) {
     using C = Cfg<TN>;
     static bool configured[64] = {};
-    qmm_status s = allow_smem(mx4_gemm_kernel<TN>, C::kSmemBytes, configured);
+    qmm_status s = allow_smem(mx4_gemm_kernel<TN, TMA>, C::kSmemBytes, configured);
     if (s != QMM_OK) return s;
     Problem q;
     s = make_problem(q, w, x, ep, y, kTM, TN, TN);
@@ -731,16 +810,17 @@ static qmm_status launch_gemm(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epil
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, mx4_gemm_kernel<TN>, q.a, q.b, q.y, q.res, q.p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, mx4_gemm_kernel<TN, TMA>, q.a, q.b, q.y, q.res, q.p);
     count_launch();
     if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? QMM_OK : cuda_fail(e, "mxfp4 gemm launch");
 }
 
+template <bool TMA>
 static qmm_status launch_gemm_pair(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epilogue &ep, uint16_t *y, cudaStream_t st) {
     using C = PairCfg;
     static bool configured[64] = {};
-    qmm_status s = allow_smem(mx4_gemm_pair_kernel, C::kSmemBytes, configured);
+    qmm_status s = allow_smem(mx4_gemm_pair_kernel<TMA>, C::kSmemBytes, configured);
     if (s != QMM_OK) return s;
     Problem q;
     s = make_problem(q, w, x, ep, y, 2 * kTM, C::kTN, C::kTN / 2);
@@ -763,7 +843,7 @@ static qmm_status launch_gemm_pair(const qmm_mx4 &w, const qmm_mx4 &x, const qmm
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, mx4_gemm_pair_kernel, q.a, q.b, sfa, sfb, q.y, q.res, q.p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, mx4_gemm_pair_kernel<TMA>, q.a, q.b, sfa, sfb, q.y, q.res, q.p);
     count_launch();
     if (e == cudaSuccess) e = cudaGetLastError();
     return e == cudaSuccess ? QMM_OK : cuda_fail(e, "mxfp4 gemm launch");
@@ -772,11 +852,25 @@ static qmm_status launch_gemm_pair(const qmm_mx4 &w, const qmm_mx4 &x, const qmm
 // Few tokens or few tiles: the kernel that splits k.  Pairs where their 256 x 256
 // tiles fill at least half of the SM pairs; below that the 128 x 192 tiles keep more
 // SMs busy.
+// Whether pairs of CTAs take the product in less time: turns of tiles over the device,
+// each as long as its products, 2.0 ns a column of k with either tile, or, where k is
+// short, its epilogue: 4.3 us (5.9 with an activation) for a CTA of a pair, 2.35 (3.4)
+// for 128 x 192.  B200, pairs against single CTAs, without and with an activation:
+// 16384 x 1024 -> 12288 182 (240) us against 131 (193), x 3072 264 (281) against 306
+// (305); 700 x 3000 -> 9000, two turns of either, 17.3 against 15.2.
+static bool pairs_take(int64_t m, int64_t k, int64_t n, bool act) {
+    auto turns = [](int64_t tiles, int64_t places) { return (tiles + places - 1) / places; };
+    const int64_t pair = turns(((m + 255) / 256) * ((n + 255) / 256), std::max(1, sm_count() / 2));
+    const int64_t single = turns(((m + kTM - 1) / kTM) * ((n + 191) / 192), sm_count());
+    return pair * std::max<int64_t>(k, act ? 3000 : 2150) < single * std::max<int64_t>(k, act ? 1700 : 1180);
+}
+
 static qmm_status launch_product(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epilogue &ep, uint16_t *y, cudaStream_t st) {
     if (mx4_small_fits(w.rows, x.rows)) return launch_mx4_small(w, nullptr, 0, 0, x, ep, y, st);
-    const int64_t pair_tiles = ((x.rows + 255) / 256) * ((w.rows + 255) / 256);
-    if (pair_tiles * 4 >= sm_count()) return launch_gemm_pair(w, x, ep, y, st);
-    return launch_gemm<192>(w, x, ep, y, st);
+    const bool tma = by_tma(w.rows);
+    if (pairs_take(x.rows, w.k, w.rows, ep.activation != QMM_ACT_NONE))
+        return tma ? launch_gemm_pair<true>(w, x, ep, y, st) : launch_gemm_pair<false>(w, x, ep, y, st);
+    return tma ? launch_gemm<192, true>(w, x, ep, y, st) : launch_gemm<192, false>(w, x, ep, y, st);
 }
 
 }  // namespace mx4

@@ -430,13 +430,13 @@ bool mx4_small_fits(int64_t n, int64_t m) {
 }
 
 bool mx4_small_quantises(int64_t n, int64_t m, int64_t k) {
-    // Every tile of features quantises its columns of x for itself.  Up to five rows
-    // of a stage a warp that is shorter than two launches (B200, 4 x 3072 -> 9216: 7.6
-    // us against 8.2; 37 x 1152 -> 3456, five a warp: 9.2 us a call against 12.7, though
-    // 8.9 against 7.9 on the device alone).
+    // Every tile of features quantises its columns of x for itself.  Up to six rows of
+    // a stage a warp a call is shorter that way than with a pass over x before it (B200,
+    // 8 x 3072 -> 9216, six a warp: 9.7 us against 10.3; 37 x 1152 -> 3456, twelve: 11.2
+    // against 9.3).
     const qmm_mx4 w{nullptr, nullptr, n, k};
     const int64_t nkb = (k + kBK - 1) / kBK, split = small::split_for(small::tiles_for(w, m), nkb, kSms);
-    return (nkb + split - 1) / split * std::min<int64_t>(m, small::tile_for(m)) <= 5 * small::kWorkers;
+    return (nkb + split - 1) / split * std::min<int64_t>(m, small::tile_for(m)) <= 6 * small::kWorkers;
 }
 
 qmm_status launch_mx4_small(const qmm_mx4 &w, const void *x, int32_t elem, int64_t x_row_stride, const qmm_mx4 &xq, const qmm_epilogue &ep,

@@ -214,6 +214,26 @@ def test_residual_in_place_bias_override_and_out(m, n):
     assert torch.equal(odd, want)
 
 
+@pytest.mark.parametrize("k", [300, 2401])  # single CTAs, pairs
+@pytest.mark.parametrize("n", [3501, 3502, 3504, 3517, 3551])  # rows of y that begin at any element; a last chunk of any width
+def test_wide_rows_at_any_alignment(k, n):
+    m = 1100
+    lin = layer(n, k, 1)
+    x = qib.mx_quantize(randn((m, k), 2).cuda())
+    xv = x.dequantize(torch.float32)
+    close(lin.forward(x), reference(lin, xv))
+    res = randn((m, n), 4, 2.0, torch.bfloat16).cuda()
+    gate = randn((n,), 3, dtype=torch.bfloat16).cuda()
+    want = lin.forward_fused(x, activation="silu", gate=gate, residual=res)
+    close(want, reference(lin, xv, "silu", gate, res))
+    close(lin.forward_fused(x, residual=res, residual_mul=True), reference(lin, xv, residual=res, mul=True))
+    guard = torch.full((m * n + 64,), 7.0, dtype=torch.bfloat16, device="cuda")
+    acc = guard[: m * n].view(m, n)
+    acc.copy_(res)
+    lin.forward_fused(x, activation="silu", gate=gate, residual=acc, out=acc)
+    assert torch.equal(acc, want) and (guard[m * n :] == 7.0).all() and qib.device_error() == 0
+
+
 def test_quantised_input_strides_batches_and_order_of_rows():
     lin = layer(300, 200, 1)
     x = randn((2, 70, 260), 2, dtype=torch.bfloat16).cuda()[:, :, 40:240]
