@@ -14,17 +14,17 @@
 // two of them).  A feature tile of 192 starts in the middle of a 128-row scale tile
 // every other time; the MMA's scale address then starts two columns in.
 //
-// Warp roles (one persistent CTA per SM): 16 epilogue warps (four per lane quadrant,
-// dealing its columns out in chunks of 32), a producer warp (TMA for codes, bulk
-// copies for scales), an MMA warp (one elected lane issues copies, MMAs and commits).  Two
+// Warp roles (one persistent CTA per SM): 12 epilogue warps (three per lane quadrant,
+// two chunks of 32 columns each; 16 share them no better and leave 96 registers a
+// thread instead of 128: 16384 x 256 -> 12288 115 us against 96), a producer warp (TMA for
+// codes, bulk copies for scales), an MMA warp (one elected lane issues copies, MMAs and commits).  Two
 // accumulators, so a tile's epilogue overlaps the next tile's main loop.  Scale
 // slots in tensor memory are tied to the shared-memory stages: a stage refilled
 // means that the MMAs that read its slot are complete.  Every wait is bounded.
 //
-// The one-CTA kernel runs where pairs (below) would leave SMs idle and k need not be
-// split (qmm_mx4_small.cu): B200, 512 x 3072 -> 3072 in 10.5 us.  At 128 x 192 its loads
-// (43 KB a stage) bound it: 4352 x 12288 -> 3072 takes 90 us here, 72 without the loads,
-// 74 on pairs.
+// Bounds (B200): with k short the epilogue (16384 x 256 -> 12288 96 us, 4.2 TB/s of y;
+// with GELU 163, its exponentials and reciprocals); with k long the loads, 43 KB a
+// stage (4352 x 12288 -> 3072 77 us, 57 on pairs, below).
 #include <algorithm>
 #include <climits>
 
@@ -34,15 +34,19 @@ namespace qmm {
 namespace mx4 {
 
 constexpr int kTM = 128;         // tokens a tile
-constexpr int kEpiWarps = 16;
-constexpr int kProducer = kEpiWarps, kMma = kEpiWarps + 1;
-constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr int kMaxChunks = 2;    // of an epilogue warp in a tile
 constexpr int kChunk = 32;       // columns an epilogue step
-constexpr int kGroups = kEpiWarps / 4;  // epilogue warps on each lane quadrant: chunk c is group c % kGroups
+
+// A CTA's warps: EPI for the epilogue, then the producer and the MMA issuer.
+template <int EPI>
+struct Warps {
+    static constexpr int kEpiWarps = EPI, kProducer = EPI, kMma = EPI + 1, kThreads = (EPI + 2) * 32;
+    static constexpr int kGroups = EPI / 4;  // epilogue warps on each lane quadrant: chunk c is group c % kGroups
+};
 
 template <int TN>
-struct Cfg {
+struct Cfg : Warps<12> {
+    using W = Warps<12>;
     static_assert(TN % 64 == 0 && TN <= 256, "feature tile");
     static constexpr int kABytes = kTM * kRowBytes;
     static constexpr int kBBytes = TN * kRowBytes;
@@ -50,8 +54,8 @@ struct Cfg {
     static constexpr int kSfaBytes = 2 * kSfTile;
     static constexpr int kSfbBytes = 2 * kBTiles * kSfTile;
     static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
-    static constexpr int kOutBytes = kEpiWarps * kChunk * 64;  // a 32 x 32 bf16 buffer a warp
-    static constexpr int kVecBytes = kEpiWarps * kMaxChunks * 2 * kChunk * 4;  // bias and gate of a warp's chunks
+    static constexpr int kOutBytes = W::kEpiWarps * kChunk * 64;  // a 32 x 32 bf16 buffer a warp
+    static constexpr int kVecBytes = W::kEpiWarps * kMaxChunks * 2 * kChunk * 4;  // bias and gate of a warp's chunks
     static constexpr int kSfCols = 2 * 4 * (1 + kBTiles);          // tensor-memory columns of a stage's scales
     static constexpr int kFit = (232448 - 1024 - 512 - kOutBytes - kVecBytes) / kStageBytes;
     static constexpr int kSlots = (512 - 2 * TN) / kSfCols;
@@ -63,7 +67,7 @@ struct Cfg {
     static constexpr int kSfbOff = kSfaOff + kStages * kSfaBytes;
     static constexpr int kVecOff = kSfbOff + kStages * kSfbBytes;
     static constexpr int kBarOff = kVecOff + kVecBytes;
-    static constexpr int kNumBars = 2 * kStages + 4 + 1 + kEpiWarps;
+    static constexpr int kNumBars = 2 * kStages + 4 + 1 + W::kEpiWarps;
     static constexpr int kSmemBytes = kBarOff + kNumBars * 8 + 16 + 1024;
     static constexpr int kSfCol0 = 2 * TN;
     static_assert(kStages >= 2 && kSmemBytes <= 232448, "shared memory");
@@ -325,7 +329,7 @@ __device__ __forceinline__ bool tile_epilogue(const Params &p, const CUtensorMap
 }
 
 template <int TN, bool TMA>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<TN>::kThreads, 1)
     mx4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                     const __grid_constant__ CUtensorMap tmap_y, const __grid_constant__ CUtensorMap tmap_res, const Params p) {
     using C = Cfg<TN>;
@@ -338,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *acc_empty = acc_full + 2;                                // [2]
     uint64_t *drain = acc_empty + 2;
     uint64_t *res_full = drain + 1;                                    // [warp] residual chunk landed
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_full + kEpiWarps);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_full + C::kEpiWarps);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
@@ -348,17 +352,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], kEpiWarps);
+            mbar_init(&acc_empty[b], C::kEpiWarps);
         }
         mbar_init(drain, 1);
-        for (int i = 0; i < kEpiWarps; ++i) mbar_init(&res_full[i], 1);
+        for (int i = 0; i < C::kEpiWarps; ++i) mbar_init(&res_full[i], 1);
         fence_barrier_init();
     }
-    if (warp == kMma) {
+    if (warp == C::kMma) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
-    if (warp == kProducer && lane == 0) {
+    if (warp == C::kProducer && lane == 0) {
         tma_prefetch_desc(&tmap_a);
         tma_prefetch_desc(&tmap_b);
         if (TMA) tma_prefetch_desc(&tmap_y);
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *tmem_slot;
     const int tiles = p.m_tiles * p.n_tiles;
 
-    if (warp == kProducer) {
+    if (warp == C::kProducer) {
         // ------------------------------------------------------------ producer
         pdl_dependency_wait();
         uint32_t i = 0;
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t first = i > (uint32_t)S ? i - S : 0;
             for (uint32_t j = first; j < i; ++j) mbar_wait(&full[j % S], (j / S) & 1, p.err, kErrTimeoutDrain);
         }
-    } else if (warp == kMma) {
+    } else if (warp == C::kMma) {
         // ------------------------------------------------------------ MMA issuer
         bool ok = true, issued = false;
         uint32_t i = 0;
@@ -473,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tile_at(p, t, mt, nt);
             const int m0 = mt * kTM + quad * 32, n0 = nt * TN;
             const int b = lt & 1;
-            auto place = [&](int c) { return kChunk * (kGroups * c + group); };
+            auto place = [&](int c) { return kChunk * (C::kGroups * c + group); };
             auto feature = [&](int c) { return place(c) < TN ? n0 + place(c) : INT_MAX - kChunk; };
             auto column = [&](int c) { return ((uint32_t)(quad * 32) << 16) + b * TN + place(c); };
             auto loaded = [&](int c) {
@@ -488,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == kMma) {
+    if (warp == C::kMma) {
         tc_fence_after_sync();
         tmem_dealloc(tmem, 512);
     }
@@ -508,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // 512 columns of tensor memory, so the accumulators share 120 columns: [0, 256) and
 // [136, 392).  The epilogue takes the half of a tile that holds them first, and the
 // next tile's main loop starts once it is in registers.
-struct PairCfg {
+struct PairCfg : Warps<16> {
     static constexpr int kTN = 256;
     static constexpr int kABytes = kTM * kRowBytes;
     static constexpr int kBBytes = kTN / 2 * kRowBytes;
@@ -558,7 +562,7 @@ __device__ __forceinline__ void tma_load_3d_pair(void *dst, const CUtensorMap *m
 }
 
 template <bool TMA>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(PairCfg::kThreads, 1)
     mx4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                          const __grid_constant__ CUtensorMap tmap_sfa, const __grid_constant__ CUtensorMap tmap_sfb,
                          const __grid_constant__ CUtensorMap tmap_y, const __grid_constant__ CUtensorMap tmap_res, const Params p) {
@@ -573,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *shared_cols = acc_empty + 2;                             // leader: a tile's shared columns are in registers
     uint64_t *drain = shared_cols + 1;
     uint64_t *res_full = drain + 1;                                    // [warp] residual chunk landed
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_full + kEpiWarps);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(res_full + C::kEpiWarps);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
@@ -586,18 +590,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&acc_full[b], 1);
-            mbar_init(&acc_empty[b], 2 * kEpiWarps);
+            mbar_init(&acc_empty[b], 2 * C::kEpiWarps);
         }
-        mbar_init(shared_cols, 2 * kEpiWarps);
+        mbar_init(shared_cols, 2 * C::kEpiWarps);
         mbar_init(drain, 1);
-        for (int i = 0; i < kEpiWarps; ++i) mbar_init(&res_full[i], 1);
+        for (int i = 0; i < C::kEpiWarps; ++i) mbar_init(&res_full[i], 1);
         fence_barrier_init();
     }
-    if (warp == kMma) {
+    if (warp == C::kMma) {
         tmem_alloc_pair(tmem_slot, 512);
         tmem_relinquish_pair();
     }
-    if (warp == kProducer && lane == 0) {
+    if (warp == C::kProducer && lane == 0) {
         tma_prefetch_desc(&tmap_a);
         tma_prefetch_desc(&tmap_b);
         tma_prefetch_desc(&tmap_sfa);
@@ -612,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *tmem_slot;
     const int tiles = p.m_tiles * p.n_tiles;
 
-    if (warp == kProducer) {
+    if (warp == C::kProducer) {
         // ------------------------------------------------------------ producer
         pdl_dependency_wait();
         uint32_t i = 0;
@@ -643,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t first = i > (uint32_t)S ? i - S : 0;
             for (uint32_t j = first; j < i; ++j) mbar_wait<true>(&full[j % S], (j / S) & 1, p.err, kErrTimeoutDrain);
         }
-    } else if (warp == kMma) {
+    } else if (warp == C::kMma) {
         // ------------------------------------------------------------ MMA issuer
         if (leader) {
             bool ok = true, issued = false;
@@ -713,7 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int m0 = mt * (2 * kTM) + (int)rank * kTM + quad * 32, n0 = nt * TN;
             const int b = lt & 1;
             // The upper half first in the first accumulator, the lower half in the second: the shared columns are among them.
-            auto place = [&](int c) { return kChunk * (kGroups * (b ? c : 1 - c) + group); };
+            auto place = [&](int c) { return kChunk * (C::kGroups * (b ? c : 1 - c) + group); };
             auto feature = [&](int c) { return n0 + place(c); };
             auto column = [&](int c) { return ((uint32_t)(quad * 32) << 16) + (b ? C::kAcc1 : 0) + place(c); };
             auto loaded = [&](int c) {
@@ -728,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before_sync();
     __syncthreads();
     cluster_sync();  // the peer's arrivals, copies and MMAs on this CTA are over
-    if (warp == kMma) {
+    if (warp == C::kMma) {
         tc_fence_after_sync();
         tmem_dealloc_pair(tmem, 512);
     }
@@ -803,7 +807,7 @@ static qmm_status launch_gemm(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epil
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     cfg.gridDim = dim3(grid, 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmemBytes;
     cfg.stream = st;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -832,7 +836,7 @@ static qmm_status launch_gemm_pair(const qmm_mx4 &w, const qmm_mx4 &x, const qmm
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3(pairs * 2, 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3(C::kThreads, 1, 1);
     cfg.dynamicSmemBytes = C::kSmemBytes;
     cfg.stream = st;
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -854,15 +858,15 @@ static qmm_status launch_gemm_pair(const qmm_mx4 &w, const qmm_mx4 &x, const qmm
 // SMs busy.
 // Whether pairs of CTAs take the product in less time: turns of tiles over the device,
 // each as long as its products, 2.0 ns a column of k with either tile, or, where k is
-// short, its epilogue: 4.3 us (5.9 with an activation) for a CTA of a pair, 2.35 (3.4)
-// for 128 x 192.  B200, pairs against single CTAs, without and with an activation:
-// 16384 x 1024 -> 12288 182 (240) us against 131 (193), x 3072 264 (281) against 306
-// (305); 700 x 3000 -> 9000, two turns of either, 17.3 against 15.2.
+// short, its epilogue: 4.3 us (7 with an activation) for a CTA of a pair, 1.7 (2.9) for
+// 128 x 192.  B200, pairs against single CTAs, without and with an activation: 16384 x
+// 1536 -> 12288 190 (249) us against 172 (180), x 3072 264 (281) against 306 (331); 2000 x
+// 3000 -> 5000, three turns of either, 23.6 against 20.5.
 static bool pairs_take(int64_t m, int64_t k, int64_t n, bool act) {
     auto turns = [](int64_t tiles, int64_t places) { return (tiles + places - 1) / places; };
     const int64_t pair = turns(((m + 255) / 256) * ((n + 255) / 256), std::max(1, sm_count() / 2));
     const int64_t single = turns(((m + kTM - 1) / kTM) * ((n + 191) / 192), sm_count());
-    return pair * std::max<int64_t>(k, act ? 3000 : 2150) < single * std::max<int64_t>(k, act ? 1700 : 1180);
+    return pair * std::max<int64_t>(k, act ? 3500 : 2150) < single * std::max<int64_t>(k, act ? 1450 : 850);
 }
 
 static qmm_status launch_product(const qmm_mx4 &w, const qmm_mx4 &x, const qmm_epilogue &ep, uint16_t *y, cudaStream_t st) {
