@@ -34,19 +34,19 @@ namespace qmm {
 namespace mx4 {
 
 constexpr int kTM = 128;         // tokens a tile
-constexpr int kMaxChunks = 2;    // of an epilogue warp in a tile
 constexpr int kChunk = 32;       // columns an epilogue step
 
 // A CTA's warps: EPI for the epilogue, then the producer and the MMA issuer.
-template <int EPI>
+template <int EPI, int CHUNKS>
 struct Warps {
+    static constexpr int kMaxChunks = CHUNKS;  // of an epilogue warp in a tile
     static constexpr int kEpiWarps = EPI, kProducer = EPI, kMma = EPI + 1, kThreads = (EPI + 2) * 32;
     static constexpr int kGroups = EPI / 4;  // epilogue warps on each lane quadrant: chunk c is group c % kGroups
 };
 
 template <int TN>
-struct Cfg : Warps<12> {
-    using W = Warps<12>;
+struct Cfg : Warps<12, 2> {
+    using W = Warps<12, 2>;
     static_assert(TN % 64 == 0 && TN <= 256, "feature tile");
     static constexpr int kABytes = kTM * kRowBytes;
     static constexpr int kBBytes = TN * kRowBytes;
@@ -55,7 +55,7 @@ struct Cfg : Warps<12> {
     static constexpr int kSfbBytes = 2 * kBTiles * kSfTile;
     static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
     static constexpr int kOutBytes = W::kEpiWarps * kChunk * 64;  // a 32 x 32 bf16 buffer a warp
-    static constexpr int kVecBytes = W::kEpiWarps * kMaxChunks * 2 * kChunk * 4;  // bias and gate of a warp's chunks
+    static constexpr int kVecBytes = W::kEpiWarps * W::kMaxChunks * 2 * kChunk * 4;  // bias and gate of a warp's chunks
     static constexpr int kSfCols = 2 * 4 * (1 + kBTiles);          // tensor-memory columns of a stage's scales
     static constexpr int kFit = (232448 - 1024 - 512 - kOutBytes - kVecBytes) / kStageBytes;
     static constexpr int kSlots = (512 - 2 * TN) / kSfCols;
@@ -282,7 +282,7 @@ __device__ __forceinline__ void chunk_finish(const Params &p, const CUtensorMap 
 
 // A tile's chunks of one warp.  feature(c): the c-th chunk's first feature (p.n or more: none); column(c): its accumulator
 // column; loaded(c) runs once chunk c is in registers; q counts the warp's chunks so far.  False: a wait ran out.
-template <bool CLUSTER, bool TMA, typename Feature, typename Column, typename Loaded>
+template <bool CLUSTER, bool TMA, int kMaxChunks, typename Feature, typename Column, typename Loaded>
 __device__ __forceinline__ bool tile_epilogue(const Params &p, const CUtensorMap *tmap_y, const CUtensorMap *tmap_res, const ChunkOut &o, uint64_t *acc_full,
                                               uint32_t parity, uint32_t tmem, int m0, uint32_t &q, const Feature &feature, const Column &column,
                                               const Loaded &loaded) {
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, 1)
         // ------------------------------------------------------------ epilogue
         pdl_dependency_wait();
         const int quad = warp & 3, group = warp >> 2;
-        const ChunkOut o{smem + C::kOutOff + warp * kChunk * 64, reinterpret_cast<float *>(smem + C::kVecOff) + warp * kMaxChunks * 2 * kChunk,
+        const ChunkOut o{smem + C::kOutOff + warp * kChunk * 64, reinterpret_cast<float *>(smem + C::kVecOff) + warp * C::kMaxChunks * 2 * kChunk,
                          res_full + warp};
         uint32_t q = 0;
         int lt = 0;
@@ -481,12 +481,12 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, 1)
             auto feature = [&](int c) { return place(c) < TN ? n0 + place(c) : INT_MAX - kChunk; };
             auto column = [&](int c) { return ((uint32_t)(quad * 32) << 16) + b * TN + place(c); };
             auto loaded = [&](int c) {
-                if (c + 1 < kMaxChunks) return;
+                if (c + 1 < C::kMaxChunks) return;
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&acc_empty[b]);
             };
-            if (!tile_epilogue<false, TMA>(p, &tmap_y, &tmap_res, o, &acc_full[b], (lt >> 1) & 1, tmem, m0, q, feature, column, loaded)) break;
+            if (!tile_epilogue<false, TMA, C::kMaxChunks>(p, &tmap_y, &tmap_res, o, &acc_full[b], (lt >> 1) & 1, tmem, m0, q, feature, column, loaded)) break;
         }
         if (lane == 0) bulk_wait_all();
     }
@@ -503,16 +503,17 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, 1)
 // features, each CTA holding 128 tokens and half of the features in its shared
 // memory and accumulating its tokens for all of them.  Against the 128 x 192 tile
 // of one CTA this reads 35 KB instead of 43 KB of operands for 1.33 times the
-// work, and spreads six scale copies over it.  B200, back to back: 4352 x 12288 x
-// 3072 74 us (4.45 PFLOP/s; one-CTA tiles 90), 16384 x 3072 x 12288 323 us, with GELU
-// 340 (369, 459).  Without its loads the first runs in 58 us, without its epilogue
-// in 68, without both in 54: operands out of L2 and the power they cost bound it.
+// work, and spreads six scale copies over it.  B200, back to back: 4352 x 12288 ->
+// 3072 57 us (5.8 PFLOP/s; one-CTA tiles 77), 16384 x 3072 -> 12288 257 us, with GELU
+// 277 (309, 332), without the epilogue's work 220: operands out of L2 and the power
+// that all of it costs bound it.  16 epilogue warps of 96 registers took 291 with GELU.
 //
 // Two accumulators of 256 columns and a scale slot for each stage do not fit the
-// 512 columns of tensor memory, so the accumulators share 120 columns: [0, 256) and
-// [136, 392).  The epilogue takes the half of a tile that holds them first, and the
-// next tile's main loop starts once it is in registers.
-struct PairCfg : Warps<16> {
+// 512 columns of tensor memory, so the accumulators share 96 columns, [0, 256) and
+// [160, 416), and four scale slots serve five stages.  The epilogue takes the chunks
+// that hold the shared columns first, and the next tile's main loop starts once they
+// are in registers.
+struct PairCfg : Warps<12, 3> {
     static constexpr int kTN = 256;
     static constexpr int kABytes = kTM * kRowBytes;
     static constexpr int kBBytes = kTN / 2 * kRowBytes;
@@ -520,11 +521,11 @@ struct PairCfg : Warps<16> {
     static constexpr int kStageBytes = kABytes + kBBytes + kSfaBytes + kSfbBytes;
     static constexpr int kOutBytes = kEpiWarps * kChunk * 64;
     static constexpr int kVecBytes = kEpiWarps * kMaxChunks * 2 * kChunk * 4;
-    static constexpr int kStages = 5;
+    static constexpr int kStages = 5, kSlots = 4;
     static constexpr int kSfCols = 24;
-    static constexpr int kAcc1 = 512 - kStages * kSfCols - kTN;  // 136
-    static constexpr int kSfCol0 = kAcc1 + kTN;                  // 392
-    static_assert(kAcc1 >= kTN / 2, "the halves drained first hold every shared column");
+    static constexpr int kAcc1 = 512 - kSlots * kSfCols - kTN;  // 160
+    static constexpr int kSfCol0 = kAcc1 + kTN;                 // 416
+    static_assert(kTN - kAcc1 <= kGroups * kChunk, "the first chunks hold every shared column");
     static constexpr int kAOff = 0;
     static constexpr int kBOff = kAOff + kStages * kABytes;
     static constexpr int kOutOff = kBOff + kStages * kBBytes;
@@ -668,11 +669,13 @@ __global__ void __launch_bounds__(PairCfg::kThreads, 1)
                 for (int kb = 0; kb < p.nkb; ++kb, ++i) {
                     const uint32_t s = i % S;
                     ok = mbar_wait<true>(&full[s], (i / S) & 1, p.err, kErrTimeoutMma);
+                    // The slot's last MMAs, kSlots stages ago, are complete.
+                    if (ok && i >= C::kSlots) ok = mbar_wait<true>(&empty[(i - C::kSlots) % S], ((i - C::kSlots) / S) & 1, p.err, kErrTimeoutMma);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     tc_fence_after_sync();
                     if (lane_elect()) {
-                        const uint32_t sfa = tmem + C::kSfCol0 + s * C::kSfCols, sfb = sfa + 8;
+                        const uint32_t sfa = tmem + C::kSfCol0 + i % C::kSlots * C::kSfCols, sfb = sfa + 8;
                         const uint64_t ad = adesc0 + (uint64_t)s * (C::kABytes >> 4), bd = bdesc0 + (uint64_t)s * (C::kBBytes >> 4);
                         const uint64_t sad = sadesc0 + (uint64_t)s * (C::kSfaBytes >> 4), sbd = sbdesc0 + (uint64_t)s * (C::kSfbBytes >> 4);
 #pragma unroll
@@ -707,7 +710,7 @@ __global__ void __launch_bounds__(PairCfg::kThreads, 1)
         // ------------------------------------------------------------ epilogue
         pdl_dependency_wait();
         const int quad = warp & 3, group = warp >> 2;
-        const ChunkOut o{smem + C::kOutOff + warp * kChunk * 64, reinterpret_cast<float *>(smem + C::kVecOff) + warp * kMaxChunks * 2 * kChunk,
+        const ChunkOut o{smem + C::kOutOff + warp * kChunk * 64, reinterpret_cast<float *>(smem + C::kVecOff) + warp * C::kMaxChunks * 2 * kChunk,
                          res_full + warp};
         uint32_t q = 0;
         int lt = 0;
@@ -716,16 +719,20 @@ __global__ void __launch_bounds__(PairCfg::kThreads, 1)
             tile_at(p, t, mt, nt);
             const int m0 = mt * (2 * kTM) + (int)rank * kTM + quad * 32, n0 = nt * TN;
             const int b = lt & 1;
-            // The upper half first in the first accumulator, the lower half in the second: the shared columns are among them.
-            auto place = [&](int c) { return kChunk * (C::kGroups * (b ? c : 1 - c) + group); };
-            auto feature = [&](int c) { return n0 + place(c); };
+            // From the last chunk down in the first accumulator, from the first up in the second: the shared columns are
+            // the first that are taken.
+            auto place = [&](int c) {
+                const int i = C::kGroups * c + group;
+                return kChunk * (b ? i : TN / kChunk - 1 - i);
+            };
+            auto feature = [&](int c) { return C::kGroups * c + group < TN / kChunk ? n0 + place(c) : INT_MAX - kChunk; };
             auto column = [&](int c) { return ((uint32_t)(quad * 32) << 16) + (b ? C::kAcc1 : 0) + place(c); };
             auto loaded = [&](int c) {
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(c == 0 ? shared_cols : &acc_empty[b]), 0));
+                if (lane == 0 && c != 1) mbar_arrive_cluster(mapa_shared(smem_u32(c == 0 ? shared_cols : &acc_empty[b]), 0));
             };
-            if (!tile_epilogue<true, TMA>(p, &tmap_y, &tmap_res, o, &acc_full[b], (lt >> 1) & 1, tmem, m0, q, feature, column, loaded)) break;
+            if (!tile_epilogue<true, TMA, C::kMaxChunks>(p, &tmap_y, &tmap_res, o, &acc_full[b], (lt >> 1) & 1, tmem, m0, q, feature, column, loaded)) break;
         }
         if (lane == 0) bulk_wait_all();
     }
