@@ -68,20 +68,20 @@ __device__ __forceinline__ float load_elem(const void *p, int elem, int64_t i) {
 // Sums over a row, spread over the CTA's warps (SLOTS at most, a multiple of four).
 // Four sets of slots taken in turn: a set is written again three barriers after its
 // readers passed theirs.  The slots of warps that are not there stay 0.
-template <int SLOTS>
+template <int SLOTS, int LANES = 32>
 struct RowSum {
     float (&red)[4][SLOTS];
     int set = 0;
     __device__ __forceinline__ RowSum(float (&r)[4][SLOTS]) : red(r) {
-        if (blockDim.x > 32) {
+        if (LANES == 32 && blockDim.x > 32) {
             for (int i = threadIdx.x; i < 4 * SLOTS; i += blockDim.x) (&red[0][0])[i] = 0.0f;
             __syncthreads();
         }
     }
     __device__ __forceinline__ float operator()(float s) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (blockDim.x > 32) {
+        for (int o = LANES / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (LANES == 32 && blockDim.x > 32) {
             if ((threadIdx.x & 31) == 0) red[set][threadIdx.x >> 5] = s;
             __syncthreads();
             s = 0.0f;
@@ -194,13 +194,13 @@ __device__ __forceinline__ void fetch_pieces(Held<BYTES, false> (&held)[VPT], ui
     }
 }
 
-// A warp's eight columns a lane, `count` in all, to any element-aligned address: through
+// Eight columns for each of LANES lanes, `count` in all, to any element-aligned address: through
 // shared memory the lanes take each other's parts of the aligned 16-byte pieces, and the
 // elements before the first (`skip` bytes) and after the last piece go one by one.
-template <typename T>
+template <int LANES, typename T>
 __device__ __forceinline__ void store_shifted(T *to, uint32_t skip, int count, const float (&v)[8], uint4 *stage) {
     constexpr int kWords = sizeof(T) * 2, kPieces = kWords / 4, kEach = 16 / sizeof(T);
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & (LANES - 1);
     uint32_t w[kWords + 4];
 #pragma unroll
     for (int k = 0; k < kWords; ++k) {
@@ -211,7 +211,7 @@ __device__ __forceinline__ void store_shifted(T *to, uint32_t skip, int count, c
 #pragma unroll
     for (int k = 0; k < kPieces; ++k) stage[lane * kPieces + k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
     __syncwarp();
-    const uint4 next = stage[min(lane + 1, 31) * kPieces];  // (lane 31 has whole pieces only where nothing is shifted)
+    const uint4 next = stage[min(lane + 1, LANES - 1) * kPieces];  // (the last lane has whole pieces only where nothing is shifted)
     w[kWords] = next.x, w[kWords + 1] = next.y, w[kWords + 2] = next.z, w[kWords + 3] = next.w;
     const int head = min((int)(skip / sizeof(T)), count), body = (count - head) / kEach;
     shift_words<kWords, sizeof(T) == 2>(w, skip);
@@ -226,14 +226,15 @@ __device__ __forceinline__ void store_shifted(T *to, uint32_t skip, int count, c
 // blockDim.x threads a row, blockDim.y rows side by side (more than one only with 32
 // threads a row).  VEC: x and branch rows, and outputs, 16-byte aligned, hidden a
 // multiple of 8.
-template <typename T, int BBYTES, int VPT, int MAXT, int MINB, bool VEC>
+template <typename T, int BBYTES, int VPT, int MAXT, int MINB, bool VEC, int LANES>
 __global__ void __launch_bounds__(MAXT, MINB)
     gated_norm_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group, const uint32_t rows_each, const bool vec_aligned) {
     extern __shared__ float4 shared_vectors[];  // A, S, H of each row side by side: threads * VPT * 8 columns (0 past the row), every thread's its own
     __shared__ __align__(16) float red[4][MAXT / 32];
     __shared__ uint4 stage[VEC ? 1 : MAXT / 32][VEC ? 1 : 16 * sizeof(T)];  // a warp's own
-    RowSum<MAXT / 32> row_sum{red};
-    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31;
+    RowSum<MAXT / 32, LANES> row_sum{red};
+    const int tid = threadIdx.x, threads = LANES == 16 ? 16 : blockDim.x, lane = tid & (LANES - 1);
+    bool live = true;  // this row is one (both halves of a warp take as many turns)
     const int hidden = (int)a.hidden;
     const float inv_hidden = 1.0f / (float)hidden;
     auto column = [&](int i) { return (i * threads + tid) * 8; };
@@ -303,10 +304,10 @@ __global__ void __launch_bounds__(MAXT, MINB)
             const float w[8] = {v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y, v[i][2].x, v[i][2].y, v[i][3].x, v[i][3].y};
             const int c = column(i);
             if constexpr (VEC) {
-                if (c < hidden) store_vec8(o + c, w);
+                if (c < hidden && live) store_vec8(o + c, w);
             } else {
                 const int from = c - lane * 8;  // the warp's first column
-                if (from < hidden) store_shifted(o + from, skip, min(256, hidden - from), w, stage[threadIdx.y + (tid >> 5)]);
+                if (from < hidden) store_shifted<LANES>(o + from, skip, live ? min(8 * LANES, hidden - from) : 0, w, &stage[0][0] + (threadIdx.y + tid / LANES) * (LANES * XB / 2));
             }
         }
     };
@@ -424,8 +425,10 @@ __global__ void __launch_bounds__(MAXT, MINB)
     const uint32_t first = (blockIdx.x * blockDim.y + threadIdx.y) * rows_each, last = min(first + rows_each, (uint32_t)a.rows);
     if (first < last) fetch(first);
     uint32_t group_end = first;
-    for (uint32_t row = first; row < last; ++row) {
-        if (row == group_end) {
+    const uint32_t end = LANES == 16 ? first + rows_each : last;
+    for (uint32_t row = first; row < end; ++row) {
+        if constexpr (LANES == 16) live = row < last;
+        if (live && row == group_end) {
             const uint32_t group = row / rows_per_group;
             group_end = (group + 1) * rows_per_group;
             take_vectors(group);
@@ -478,12 +481,15 @@ __global__ void __launch_bounds__(MAXT, MINB)
             const int c = column(i);
             uint32_t codes;
             const uint32_t e = mx4_encode8(w, &codes);
-            if (c / 2 < pitch) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = codes;
+            if (c / 2 < pitch && live) *reinterpret_cast<uint32_t *>(a.n_codes + row * pitch + c / 2) = codes;
             uint32_t word = e << (8 * ((lane >> 2) & 3));
             word |= __shfl_xor_sync(0xffffffffu, word, 4);
             word |= __shfl_xor_sync(0xffffffffu, word, 8);
             const int64_t b = c / kMxBlock;
-            if ((lane & 15) == 0 && b < tiles * 4) *reinterpret_cast<uint32_t *>(a.n_scales + mx4_scale_offset(row, b, tiles)) = word;
+            if ((lane & 15) == 0 && b < tiles * 4 && live) {
+                *reinterpret_cast<uint32_t *>(a.n_scales + mx4_scale_offset(row, b, tiles)) = word;
+                if (LANES == 16) *reinterpret_cast<uint32_t *>(a.n_scales + mx4_scale_offset(row, 4, tiles)) = 0;
+            }
         }
     }
 }
@@ -561,11 +567,11 @@ static unsigned threads_for(int64_t hidden) {
     return (unsigned)(((vectors + VPT - 1) / VPT + 31) / 32 * 32);
 }
 
-template <typename T, int BBYTES, int VPT, int MAXT, int MINB, bool VEC>
+template <typename T, int BBYTES, int VPT, int MAXT, int MINB, bool VEC, int LANES = 32>
 static cudaError_t launch_rows(const qmm_gated_norm_args &a, uint32_t rpg, bool vec_aligned, cudaStream_t st) {
-    auto kernel = gated_norm_kernel<T, BBYTES, VPT, MAXT, MINB, VEC>;
-    const unsigned threads = threads_for<VPT>(a.hidden);
-    const dim3 block(threads, threads == 32 ? 4 : 1, 1);
+    auto kernel = gated_norm_kernel<T, BBYTES, VPT, MAXT, MINB, VEC, LANES>;
+    const unsigned threads = LANES == 16 ? 16 : threads_for<VPT>(a.hidden);
+    const dim3 block(threads, threads <= 32 ? 128 / threads : 1, 1);
     const size_t smem = (size_t)threads * block.y * VPT * 8 * 4 * 3;
     static int resident[64][33] = {};  // CTAs an SM by device and warps a row
     int dev = 0;
@@ -591,6 +597,7 @@ static cudaError_t launch_fast(const qmm_gated_norm_args &a, uint32_t rpg, bool 
     // its registers allow at 12 warps an SM or more (B200, 16896 x 2048 bf16: two vectors
     // a thread 70 us, one 77).
     constexpr bool W = sizeof(T) == 4 || BBYTES == 4 || !VEC;  // more registers a vector
+    if (a.hidden <= 128) return launch_rows<T, BBYTES, 1, 256, W ? 3 : 4, VEC, 16>(a, rpg, vec_aligned, st);
     if (a.hidden <= 256) return launch_rows<T, BBYTES, 1, 256, W ? 3 : 4, VEC>(a, rpg, vec_aligned, st);
     if (a.hidden <= 512) return launch_rows<T, BBYTES, 2, 256, W ? 2 : 3, VEC>(a, rpg, vec_aligned, st);
     if (a.hidden <= 4096) return launch_rows<T, BBYTES, 2, 256, W ? 2 : 3, VEC>(a, rpg, vec_aligned, st);
