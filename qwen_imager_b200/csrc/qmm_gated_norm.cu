@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(MAXT, MINB)
             const float w[8] = {v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y, v[i][2].x, v[i][2].y, v[i][3].x, v[i][3].y};
             const int c = column(i);
             if constexpr (VEC) {
-                if (c < hidden && live) store_vec8(o + c, w);
+                if (c < hidden && live) store_vec8_global(o + c, w);
             } else {
                 const int from = c - lane * 8;  // the warp's first column
                 if (from < hidden) store_shifted<LANES>(o + from, skip, live ? min(8 * LANES, hidden - from) : 0, w, &stage[0][0] + (threadIdx.y + tid / LANES) * (LANES * XB / 2));

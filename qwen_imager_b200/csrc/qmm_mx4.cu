@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const DequantAr
         for (int q = 0; q < 8; ++q) v[q] *= s;
         if constexpr (VEC) {
             const int64_t c = col0 + lane * 8;
-            if (c < a.k) store_vec8(dst + r * a.k + c, v);
+            if (c < a.k) store_vec8_global(dst + r * a.k + c, v);
         } else {
             __syncwarp();
             store_vec8(&stage[warp][lane * 8], v);
