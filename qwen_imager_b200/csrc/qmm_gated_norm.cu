@@ -3,8 +3,8 @@
 //   x' = residual_scale * x + gate * h
 //   n  = norm_pre(x') * pre_weight * (1 + scale) + shift
 // HBM-bound: x and branch are read once, x' and n (or its MXFP4 codes) written
-// once.  A row stays in the registers of a warp (up to 512 columns, several rows a
-// CTA) or of a CTA, eight columns a vector, up to four vectors a thread, so mean and
+// once.  A row stays in the registers of half a warp (up to 128 columns), a warp (up to
+// 512) or a CTA, eight columns a vector, up to four vectors a thread, so mean and
 // variance are two passes over registers, and each statistic costs one shuffle tree
 // and, in a CTA, one shared slot a warp and one barrier.  The grid is what is resident
 // at once, consecutive rows to a warp or CTA; it loads its next row while it works on
@@ -12,9 +12,11 @@
 // gate, S = pre_weight * (1 + scale) and H = shift, formed once (and again where the
 // group changes) in shared memory, and arithmetic goes two columns an instruction:
 // with the vectors loaded and converted row by row the kernel was bound by its
-// instructions (16896 x 3072 bf16: 116 us against 85).
-// Rows that are not 16-byte aligned deal their columns out one by one (thread t
-// holds columns t, t + T, ...), which keeps accesses of a warp consecutive.  Rows past
+// instructions (B200, 16896 x 3072 bf16: 116 us against 85; now 72, 0.88 of the measured
+// HBM rate).  More rows on their way cost registers: two 101 us, three 103.
+// Rows that are not 16-byte aligned are read by the aligned pieces that hold them and
+// shifted into place, and stored likewise; that is bound by its instructions (4096 x
+// 1677 28 us, 0.30 of HBM, x 1680 16; one element a lane at a time took 52).  Rows past
 // 16384 columns, whose vectors do not fit, take a kernel without them.
 #include <algorithm>
 #include <type_traits>
@@ -593,9 +595,9 @@ static cudaError_t launch_rows(const qmm_gated_norm_args &a, uint32_t rpg, bool 
 
 template <typename T, int BBYTES, bool VEC>
 static cudaError_t launch_fast(const qmm_gated_norm_args &a, uint32_t rpg, bool vec_aligned, cudaStream_t st) {
-    // A warp a row where its lanes hold it; then a CTA, with as many vectors a thread as
-    // its registers allow at 12 warps an SM or more (B200, 16896 x 2048 bf16: two vectors
-    // a thread 70 us, one 77).
+    // Half a warp or a warp a row where its lanes hold it (B200, 30000 x 128 bf16: half a
+    // warp 8.7 us, a warp 14.6); then a CTA, with as many vectors a thread as its registers
+    // allow at 12 warps an SM or more (16896 x 2048: two vectors a thread 70 us, one 77).
     constexpr bool W = sizeof(T) == 4 || BBYTES == 4 || !VEC;  // more registers a vector
     if (a.hidden <= 128) return launch_rows<T, BBYTES, 1, 256, W ? 3 : 4, VEC, 16>(a, rpg, vec_aligned, st);
     if (a.hidden <= 256) return launch_rows<T, BBYTES, 1, 256, W ? 3 : 4, VEC>(a, rpg, vec_aligned, st);

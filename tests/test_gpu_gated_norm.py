@@ -130,6 +130,42 @@ def test_in_place_and_strided_rows(hidden):
     assert r[0] is x2 and r[1] is b2 and torch.equal(x2, want[0]) and torch.equal(b2, want[1])
 
 
+@pytest.mark.parametrize("xt,bt", [(BF, BF), (torch.float16, BF), (torch.float32, BF), (torch.float32, torch.float32), (BF, torch.float32)])
+@pytest.mark.parametrize("rows,hidden", [(1, 1), (9, 3), (30, 84), (31, 127), (5, 129), (40, 201), (12, 257), (6, 511), (7, 1677), (3, 5001), (2, 9001)])
+@pytest.mark.parametrize("at,gap", [(0, 0), (1, 0), (3, 2), (6, 10)])  # first column, columns between rows
+def test_rows_at_any_alignment_among_nan(rows, hidden, xt, bt, at, gap):
+    x, b, s = make(rows, hidden, xt, bt, groups=1 if rows % 2 else 2)
+
+    def slot(t, dtype, fill):  # t as a view inside a buffer of `fill`
+        buf = torch.full((at + rows * (hidden + gap) + 5,), fill, dtype=dtype, device="cuda")
+        view = torch.as_strided(buf, (rows, hidden), (hidden + gap, 1), at)
+        if t is not None:
+            view.copy_(t)
+        return buf, view
+
+    _, xv = slot(x, xt, math.nan)
+    _, bv = slot(b, bt, math.nan)
+    (xb, xo), (nb, no) = slot(None, xt, 7.0), slot(None, xt, 7.0)
+    qib.gated_residual_norm(xv, bv, post="rms", pre="layer", residual_scale=0.75, x_out=xo, n_out=no, **s)
+    ref = reference(x, b, s, "rms", "layer", 0.75)
+    close(xo, ref[0])
+    close(no, ref[1])
+    for buf, view in ((xb, xo), (nb, no)):
+        view.fill_(7.0)
+        assert (buf == 7.0).all()  # nothing written beside the rows
+
+
+@pytest.mark.parametrize("rows,hidden", [(33, 100), (50, 128), (7, 129), (3, 5), (129, 120)])
+def test_mxfp4_of_narrow_rows(rows, hidden):
+    x, b, s = make(rows, hidden, torch.float32, BF)
+    _, n = qib.gated_residual_norm(x, b, post="rms", pre="layer", **s)
+    _, q = qib.gated_residual_norm(x, b, post="rms", pre="layer", quantize=True, **s)
+    want = qib.mx_quantize(n)
+    assert torch.equal(q.row_scales(), want.row_scales()) and torch.equal(q.codes, want.codes)
+    lin = qib.MxLinear.from_dense(torch.randn((96, hidden), device="cuda"))
+    assert torch.equal(lin.forward(q), lin.forward(n))
+
+
 @pytest.mark.parametrize("rows,hidden", [(1, 64), (3, 40), (130, 3072), (33, 1000), (5, 761), (2, 9000)])
 def test_mxfp4_result_is_the_quantised_norm(rows, hidden):
     x, b, s = make(rows, hidden, torch.float32, BF)
