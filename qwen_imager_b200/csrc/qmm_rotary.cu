@@ -5,8 +5,9 @@
 // token.  A warp takes a token and a run of its heads.  Each lane holds the same
 // four pairs of every head (as two runs of four columns), so the token's sines
 // and cosines, computed once in the warp (a pair or two a lane, handed round by
-// shuffles) and multiplied with the norm's weight, stay in registers over the heads; a head of 8 U columns takes U lanes, and
-// 32 / U heads (rounded down) go at a time.  Arithmetic goes two columns an instruction.
+// shuffles) and multiplied with the norm's weight, stay in registers over the
+// heads; a head of 8 U columns takes U lanes, and 32 / U heads (rounded down) go at a
+// time.  Arithmetic goes two columns an instruction.
 //
 // The angle is positions * turns in turns.  With turns = f + g (leading and
 // trailing term), p = fl(pos f) and e = pos f - p exact by one fma, the fraction
@@ -18,7 +19,9 @@ namespace qmm {
 namespace rotary {
 
 constexpr int kWarps = 4;
-constexpr int kResident = 8;  // CTAs an SM: 32 warps cover the loads (B200, 16896 x 48 heads x 128, each lane turning its own pairs: 72.8 us; with 16 warps 94.9, with 40 78.8)
+// CTAs an SM: 32 warps cover the loads (B200, 16896 x 48 heads x 128 bf16: 70 us, 0.90 of
+// the measured HBM rate; before lanes shared their sines 73, with 16 warps 95, with 40 79).
+constexpr int kResident = 8;
 
 __device__ __forceinline__ float position_of(const qmm_rotary_args &a, int64_t batch, int64_t token, int axis) {
     const int64_t i = batch * a.pos_batch_stride + token * a.axes + axis;
