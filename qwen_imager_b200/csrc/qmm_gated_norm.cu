@@ -16,7 +16,7 @@
 // HBM rate).  More rows on their way cost registers: two 101 us, three 103.
 // Rows that are not 16-byte aligned are read by the aligned pieces that hold them and
 // shifted into place, and stored likewise; that is bound by its instructions (4096 x
-// 1677 28 us, 0.30 of HBM, x 1680 16; one element a lane at a time took 52).  Rows past
+// 1677 26 us, 0.32 of HBM, x 1680 16; one element a lane at a time took 52).  Rows past
 // 16384 columns, whose vectors do not fit, take a kernel without them.
 #include <algorithm>
 #include <type_traits>
@@ -171,23 +171,23 @@ __device__ __forceinline__ void fetch_pieces(Held<BYTES, false> (&held)[VPT], ui
 #pragma unroll
             for (int k = 0; k < kPieces; ++k)
                 held[i].piece[k] = *reinterpret_cast<const uint4 *>(a + min((first + i * step) * BYTES + 16 * k, last));
-    } else {  // the pieces at the operand's ends: one element at a time
+    } else {  // the pieces across the operand's ends: the row's elements in them, one by one
+        const int lo = (int)max((int64_t)(base - p), (int64_t)-16), length = hidden * BYTES, hi = (int)min((int64_t)(end - p), (int64_t)length + 16);
 #pragma unroll
         for (int i = 0; i < VPT; ++i)
 #pragma unroll
             for (int k = 0; k < kPieces; ++k) {
-                const uintptr_t q = a + (int64_t)(first + i * step) * BYTES + 16 * k;
+                const int off = (first + i * step) * BYTES + 16 * k - (int)(p - a);  // from the row's first byte
                 held[i].piece[k] = make_uint4(0, 0, 0, 0);
-                if (q >= base && q + 16 <= end) {
-                    held[i].piece[k] = *reinterpret_cast<const uint4 *>(q);
-                } else if (q < past) {
+                if (off >= lo && off + 16 <= hi) {
+                    held[i].piece[k] = *reinterpret_cast<const uint4 *>(p + off);
+                } else if (off < length) {
                     uint32_t w[4] = {};
 #pragma unroll
                     for (int e = 0; e < 16 / BYTES; ++e) {
-                        const uintptr_t at = q + e * BYTES;
-                        if (at >= p && at < past) {
-                            if constexpr (BYTES == 4) w[e] = *reinterpret_cast<const uint32_t *>(at);
-                            else w[e / 2] |= (uint32_t)*reinterpret_cast<const uint16_t *>(at) << (16 * (e & 1));
+                        if ((uint32_t)(off + e * BYTES) < (uint32_t)length) {
+                            if constexpr (BYTES == 4) w[e] = *reinterpret_cast<const uint32_t *>(p + off + e * BYTES);
+                            else w[e / 2] |= (uint32_t)*reinterpret_cast<const uint16_t *>(p + off + e * BYTES) << (16 * (e & 1));
                         }
                     }
                     held[i].piece[k] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -231,7 +231,7 @@ __device__ __forceinline__ void store_shifted(T *to, uint32_t skip, int count, c
 template <typename T, int BBYTES, int VPT, int MAXT, int MINB, bool VEC, int LANES>
 __global__ void __launch_bounds__(MAXT, MINB)
     gated_norm_kernel(const qmm_gated_norm_args a, const uint32_t rows_per_group, const uint32_t rows_each, const bool vec_aligned) {
-    extern __shared__ float4 shared_vectors[];  // A, S, H of each row side by side: threads * VPT * 8 columns (0 past the row), every thread's its own
+    extern __shared__ float4 shared_vectors[];  // A, S, H of each row side by side: threads * VPT * 8 columns (0 past the row), each thread's columns side by side
     __shared__ __align__(16) float red[4][MAXT / 32];
     __shared__ uint4 stage[VEC ? 1 : MAXT / 32][VEC ? 1 : 16 * sizeof(T)];  // a warp's own
     RowSum<MAXT / 32, LANES> row_sum{red};
@@ -330,9 +330,9 @@ __global__ void __launch_bounds__(MAXT, MINB)
                 o[0] = make_float4(f[0], f[1], f[2], f[3]);
                 o[threads] = make_float4(f[4], f[5], f[6], f[7]);
             };
-            if (vec_aligned && (VEC || column(i) + 8 <= hidden)) {  // every load is on its way before the first is used
+            if (vec_aligned) {  // every load is on its way before the first is used
                 const int c = column(i);
-                const bool in = c < hidden;
+                const bool in = VEC ? c < hidden : c + 8 <= hidden;
                 auto raw = [&](const void *p, int64_t at) {
                     Raw8<4> r{};
                     if (in && p) {
@@ -364,6 +364,20 @@ __global__ void __launch_bounds__(MAXT, MINB)
                 put(1, f);
                 values(r4, a.shift, 0.0f, f);
                 put(2, f);
+                const int col = (hidden & ~7) + lane;
+                if (!VEC && c - lane * 8 < hidden && (hidden & 7) != 0 && c - lane * 8 + 8 * LANES >= hidden) {  // the row's last vector: a column a lane
+                    const uint32_t lanes = LANES == 16 ? 0xFFFFu << (threadIdx.y & 1) * 16 : 0xFFFFFFFFu;
+                    __syncwarp(lanes);
+                    if (col < hidden) {
+                        auto at = [&](const void *p, int64_t base, float none) { return p ? load_elem(p, a.vec_elem, base + col) : none; };
+                        const float v = at(a.pre_weight, 0, 1.0f);
+                        float *const o = reinterpret_cast<float *>(vectors + i * threads + (col & 4 ? threads : 0) + (col >> 3)) + (col & 3);
+                        o[0] = at(a.post_weight, 0, 1.0f) * at(a.gate, gate, 1.0f);
+                        o[span * 4] = fmaf(v, at(a.scale, scale, 0.0f), v);
+                        o[span * 8] = at(a.shift, shift, 0.0f);
+                    }
+                    __syncwarp(lanes);
+                }
             } else {
                 // One element at a time, the loads of four columns on their way together.
                 auto value = [&](uint32_t w) {
