@@ -332,8 +332,8 @@ QMM_API qmm_status qmm_debug_gemm_stall(int32_t withhold_block, uint64_t wait_li
  * before it on the stream (programmatic dependent launch), so they arrive
  * while that kernel drains; x, bias, gate and residual are still read, and y
  * written, only after it has completed.  Off by default.  Applies to launches
- * made after the call, in this process; returns the previous setting.  No
- * counterpart in quant.rs.
+ * made after the call, in this process; returns the previous setting.  MXFP4
+ * products (qmm_block.h) wait whatever the setting.  No counterpart in quant.rs.
  */
 QMM_API int32_t qmm_set_weights_immutable(int32_t on);
 

@@ -84,7 +84,10 @@ QMM_API qmm_status qmm_mx4_row_scales(const uint8_t *scales, int64_t rows, int64
  * more than qmm_mx4_workspace_bytes(m, k)).  Products of codes
  * and scales are exact, sums are f32.  bias, gate bf16 [n] or NULL; residual
  * bf16 [m, n] or NULL, it may alias y.  y must not overlap x, W or workspace.
- * Calls that share a workspace must be ordered on one stream.
+ * Calls that share a workspace must be ordered on one stream.  Every operand,
+ * W among them, is read only after the kernels ahead on the stream have
+ * completed, whatever qmm_set_weights_immutable says: W may come straight out
+ * of qmm_mx4_quantize.
  */
 typedef struct qmm_mx4_linear_args {
     qmm_mx4 w;

@@ -62,7 +62,6 @@ struct Params {
     int32_t m, n, k;
     int32_t nkb, sf_tiles;   // stages along k; scale tiles along k
     int32_t vec;             // rows of x on 16-byte boundaries, k a multiple of 8
-    int32_t early;           // the weight may be read before the kernels ahead have completed
     uint32_t *err;
 };
 
@@ -164,12 +163,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                       C::kSfBytes, &full[s]);
         };
         const int first = min(S, nkb);
-        if (p.early && lane == 0)
-            for (int i = 0; i < first; ++i) copy_weight(i);
+        // The weight too: the kernel ahead may be the quantisation that makes it.
         pdl_dependency_wait();
         if (lane == 0) {
             for (int i = 0; i < first; ++i) {
-                if (!p.early) copy_weight(i);
+                copy_weight(i);
                 if (!quantise) copy_x(i);
             }
         }
@@ -377,7 +375,6 @@ static qmm_status launch(const qmm_mx4 &w, const void *x, int64_t x_row_stride, 
     p.nkb = (int32_t)((w.k + kBK - 1) / kBK);
     p.sf_tiles = (int32_t)mx4_scale_tiles(w.k);
     p.vec = w.k % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (xq.rows == 1 || (x_row_stride * (int64_t)sizeof(T)) % 16 == 0);
-    p.early = weights_immutable() ? 1 : 0;
     p.err = device_error_word();
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
