@@ -124,8 +124,12 @@ struct Heads {
 
 // A warp takes a token and a run of its q and k heads.  Needs dim % 8 == 0, with
 // halves pairs % 4 == 0, heads aligned as the layout says.  NORM: some weight is
-// given; POW2: dim / 8 is a power of two.
-template <typename T, Layout L, bool NORM, bool POW2, int kTurns>
+// given; POW2: dim / 8 is a power of two; TAIL: some columns are not turned.  A turn by 0
+// would mix an infinity or NaN of one into its lane's neighbour (0 times either is NaN),
+// so selects keep them apart (B200, 16896 x 48 x 128 with 32 of 64 pairs 71.6 -> 75.8 us, in
+// halves 77.8 -> 80.7; 2 x 14317 x 24 x 72 f16 41.0 -> 43.0; a branch on the head's sum of
+// squares and predicated products cost registers and as much time).
+template <typename T, Layout L, bool NORM, bool POW2, bool TAIL, int kTurns>
 __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qmm_rotary_args a, const int heads_per_warp) {
     constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;  // heads a lane group has in flight
     const int units = a.dim >> 3, at_a_time = 32 / units;
@@ -138,6 +142,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qm
     const int pair = u * 4;
     const int ca = L == kHalves && pair < a.pairs ? pair : u * 8, cb = L == kHalves && pair < a.pairs ? a.pairs + pair : u * 8 + 4;
     const float inv_dim = 1.0f / (float)a.dim;
+    auto turns = [&](int i) { return pair + (L == kHalves ? 0 : i) < a.pairs; };  // pair i of the lane (halves: all four or none)
     float2 cs[2], sn[2];
     bool turned = false;
 
@@ -187,6 +192,8 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qm
                     fb[i] = mul_f32x2(wo[i], make_float2(-sn[i].x, -sn[i].y));
                     fc[i] = mul_f32x2(we[i], sn[i]);
                     fd[i] = mul_f32x2(wo[i], cs[i]);
+                    if (TAIL && !turns(2 * i)) fb[i].x = fc[i].x = -0.0f;  // 0 * -0 changes no number that it is added to
+                    if (TAIL && !turns(2 * i + 1)) fb[i].y = fc[i].y = -0.0f;
                 }
             }
 #pragma unroll
@@ -222,8 +229,14 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qm
                     float2 oa[2], ob[2];
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
-                        oa[q] = fma_f32x2(x[q], fa[q], mul_f32x2(y[q], fb[q]));
-                        ob[q] = fma_f32x2(x[q], fc[q], mul_f32x2(y[q], fd[q]));
+                        float2 xc = x[q], yc = y[q];
+                        if constexpr (TAIL) {
+                            const bool first = turns(2 * q), second = turns(2 * q + 1);
+                            xc = make_float2(first ? xc.x : 0.0f, second ? xc.y : 0.0f);
+                            yc = make_float2(first ? yc.x : 0.0f, second ? yc.y : 0.0f);
+                        }
+                        oa[q] = fma_f32x2(x[q], fa[q], mul_f32x2(yc, fb[q]));
+                        ob[q] = fma_f32x2(xc, fc[q], mul_f32x2(y[q], fd[q]));
                     }
                     store_pairs<T, L>(dst + j * dst_step, ca, cb, oa, ob);
                 }
@@ -331,14 +344,16 @@ static qmm_status launch(const qmm_rotary_args &a, bool fast, bool wide, cudaStr
     const bool norm = a.q_weight || a.k_weight, pow2 = (units & (units - 1)) == 0;
 #define QMM_ROTARY(L)                                                                            \
     (a.pairs <= 32 ? QMM_ROTARY_N(L, 1) : a.pairs <= 64 ? QMM_ROTARY_N(L, 2) : QMM_ROTARY_N(L, 4))
-#define QMM_ROTARY_N(L, N)                                                                       \
-    (!norm  ? rotary_kernel<T, L, false, true, N><<<grid, kWarps * 32, 0, st>>>(a, per)          \
-     : pow2 ? rotary_kernel<T, L, true, true, N><<<grid, kWarps * 32, 0, st>>>(a, per)           \
-            : rotary_kernel<T, L, true, false, N><<<grid, kWarps * 32, 0, st>>>(a, per))
+#define QMM_ROTARY_N(L, N) (2 * a.pairs < a.dim ? QMM_ROTARY_T(L, true, N) : QMM_ROTARY_T(L, false, N))
+#define QMM_ROTARY_T(L, TAIL, N)                                                                 \
+    (!norm  ? rotary_kernel<T, L, false, true, TAIL, N><<<grid, kWarps * 32, 0, st>>>(a, per)    \
+     : pow2 ? rotary_kernel<T, L, true, true, TAIL, N><<<grid, kWarps * 32, 0, st>>>(a, per)     \
+            : rotary_kernel<T, L, true, false, TAIL, N><<<grid, kWarps * 32, 0, st>>>(a, per))
     if (!fast) rotary_any_kernel<T><<<grid, kWarps * 32, 0, st>>>(a, per);
     else if (wide) QMM_ROTARY(kWide);
     else if (a.adjacent) QMM_ROTARY(kAdjacent);
     else QMM_ROTARY(kHalves);
+#undef QMM_ROTARY_T
 #undef QMM_ROTARY_N
 #undef QMM_ROTARY
     count_launch();
