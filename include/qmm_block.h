@@ -119,8 +119,10 @@ QMM_API qmm_status qmm_mx4_linear(const qmm_mx4_linear_args *a, void *stream);
  *   (a, b) of pair p -> (a cos phi - b sin phi, a sin phi + b cos phi)
  * with (a, b) columns (2 p, 2 p + 1) of the head (adjacent) or (p, pairs + p)
  * (halves); columns from 2 * pairs on are only normalised.  f32 arithmetic,
- * one rounding.  Whole turns are dropped before the sine and cosine, so far
- * positions lose no accuracy.
+ * one rounding.  Whole turns are dropped before the sine and cosine: the angle
+ * is right to about 2^-23 turns at positions up to 2^24, whole or not, and to
+ * 2^-52 of the position in turns beyond (whole positions up to 2^48; turns up
+ * to 1 / (2 pi); 2^-21 turns at 2^31).
  *
  * q [batch, tokens, q_heads, dim] and k [batch, tokens, k_heads, dim] lie at
  * the given element strides (batch, token, head; columns are contiguous), as

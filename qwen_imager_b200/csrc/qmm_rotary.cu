@@ -11,7 +11,10 @@
 //
 // The angle is positions * turns in turns.  With turns = f + g (leading and
 // trailing term), p = fl(pos f) and e = pos f - p exact by one fma, the fraction
-// of p is exact and the angle's error stays near 2^-24 turns at any position.
+// of p is exact and the angle's error stays near 2^-24 turns up to positions of 2^24.
+// Past these a whole position is two terms too, each product gives up its whole
+// turns, and what g lacks of the frequency decides: 2^-52 of the position, for
+// frequencies up to a radian (2^-21 turns at 2^31).
 #include "qmm_internal.h"
 #include "qmm_mx4.cuh"
 
@@ -23,19 +26,33 @@ constexpr int kWarps = 4;
 // the measured HBM rate; before lanes shared their sines 73, with 16 warps 95, with 40 79).
 constexpr int kResident = 8;
 
-__device__ __forceinline__ float position_of(const qmm_rotary_args &a, int64_t batch, int64_t token, int axis) {
+// A position as two terms: whole numbers past 2^24 do not fit one.
+__device__ __forceinline__ float position_of(const qmm_rotary_args &a, int64_t batch, int64_t token, int axis, float *low) {
     const int64_t i = batch * a.pos_batch_stride + token * a.axes + axis;
-    if (a.pos_kind == 0) return (float)static_cast<const int32_t *>(a.positions)[i];
-    if (a.pos_kind == 1) return (float)static_cast<const int64_t *>(a.positions)[i];
-    return static_cast<const float *>(a.positions)[i];
+    *low = 0.0f;
+    if (a.pos_kind == 2) return static_cast<const float *>(a.positions)[i];
+    const int64_t v = a.pos_kind == 0 ? static_cast<const int32_t *>(a.positions)[i] : static_cast<const int64_t *>(a.positions)[i];
+    const float high = (float)v;
+    *low = (float)(v - (int64_t)high);
+    return high;
 }
 
+__device__ __forceinline__ float fraction(float x) { return x - rintf(x); }
+
 __device__ __forceinline__ void pair_turn(const qmm_rotary_args &a, int64_t batch, int64_t token, int pair, float *c, float *s) {
-    const float pos = position_of(a, batch, token, a.axis[pair]);
+    float low;
+    const float pos = position_of(a, batch, token, a.axis[pair], &low);
     const float f = a.turns[2 * pair], g = a.turns[2 * pair + 1];
     const float p = pos * f;
     const float e = fmaf(pos, f, -p);
-    const float t = (p - rintf(p)) + fmaf(pos, g, e);
+    float t;
+    if (fabsf(pos) <= 16777216.0f && low == 0.0f) {
+        t = fraction(p) + fmaf(pos, g, e);
+    } else {
+        const float pg = pos * g, pl = low * f;
+        const float small = fmaf(pos, g, -pg) + fmaf(low, f, -pl) + low * g;
+        t = fraction(p) + fraction(e) + fraction(pg) + fraction(pl) + small;
+    }
     sincospif(2.0f * t, s, c);
 }
 

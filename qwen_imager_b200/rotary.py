@@ -75,7 +75,8 @@ def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.
     q [tokens, heads, dim] or [batch, tokens, heads, dim], any strides with
     consecutive columns (slices of a fused projection); k likewise, its heads
     may differ, or None.  positions [tokens, axes], or [batch, tokens, axes]:
-    int32, int64 or f32 (whole numbers to 2^24 and fractions exactly).
+    int32, int64 or f32; whole turns drop out exactly, so far positions keep
+    their accuracy (include/qmm_block.h).
     Outputs are new contiguous tensors, or q_out / k_out, which may be q / k."""
     if q_out is None and k_out is None:
         made = _block.host().qk_norm_rotary(q, k, positions, axes._turns, axes._axis, axes.axes, axes._adjacent, q_weight, k_weight, eps)
