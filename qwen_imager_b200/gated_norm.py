@@ -42,7 +42,7 @@ def gated_residual_norm(x: torch.Tensor, branch: Optional[torch.Tensor] = None, 
             made = _block.checked(made)
             if not quantize:
                 return made
-            return made[0], MxTensor(made[1], made[2], made[1].shape[0], x.shape[-1], x.shape[:-1])
+            return made[0], MxTensor._made(made[1], made[2], made[1].shape[0], x.shape[-1], x.shape[:-1])
     device = _block.require_cuda(x, "x")
     x_elem = _block.elem_of(x, "x")
     post_kind, pre_kind = _block.NORMS.get(post), _block.NORMS.get(pre)

@@ -11,6 +11,7 @@ cores' block-scaled 4-bit path.  Its `forward_fused` takes the arguments of
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Union
 
 import torch
@@ -19,6 +20,7 @@ from . import _block
 from ._block import bad_argument, bad_shape
 from .quant import ACTIVATIONS, OWN_BIAS
 from . import _lib
+from ._lib import QmmError
 
 BLOCK = 32
 
@@ -26,24 +28,50 @@ _host = _block.host
 _checked = _block.checked
 
 
+def _sizes(rows: int, k: int):
+    """Shape of the codes and bytes of the scales of [rows, k]."""
+    return (rows, -(-k // BLOCK) * 16), -(-rows // 128) * -(-k // 256) * 1024
+
+
 class MxTensor:
     """An MXFP4 matrix [rows, k] (qmm_mx4 of include/qmm_block.h).
 
     codes: uint8 [rows, 16 * ceil(k / 32)], column 2 j in the low four bits of
     byte j; scales: uint8, in the order of the tensor cores (row_scales() gives
-    them as [rows, ceil(k / 32)])."""
+    them as [rows, ceil(k / 32)]).  Both contiguous, of exactly these sizes,
+    16-byte aligned and on one device; lead, whose product is rows, shapes
+    results."""
 
     __slots__ = ("codes", "scales", "rows", "k", "lead")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, rows: int, k: int, lead=None):
-        self.codes, self.scales, self.rows, self.k = codes, scales, rows, k
-        self.lead = (rows,) if lead is None else tuple(lead)  # leading dimensions of the quantised tensor
+        rows, k = int(rows), int(k)
+        lead = (rows,) if lead is None else tuple(int(n) for n in lead)  # leading dimensions of the quantised tensor
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise bad_argument(f"MXFP4 codes and scales are uint8, not {codes.dtype} and {scales.dtype}")
+        if rows < 0 or k <= 0 or math.prod(lead) != rows or any(n < 0 for n in lead):
+            raise bad_shape(f"an MXFP4 matrix of [{rows}, {k}] with leading dimensions {lead}")
+        want, tiles = _sizes(rows, k)
+        if tuple(codes.shape) != want or tuple(scales.shape) != (tiles,):
+            raise bad_shape(f"MXFP4 [{rows}, {k}] needs codes {want} and {tiles} bytes of scales, not {tuple(codes.shape)} and {tuple(scales.shape)}")
+        if codes.device != scales.device or not codes.is_contiguous() or not scales.is_contiguous():
+            raise bad_argument(f"MXFP4 codes on {codes.device} and scales on {scales.device}: both must be contiguous, on one device")
+        if codes.data_ptr() % 16 or scales.data_ptr() % 16:
+            raise QmmError(_lib.QMM_ERR_MISALIGNED, "MXFP4 codes and scales must be 16-byte aligned")
+        self.codes, self.scales, self.rows, self.k, self.lead = codes, scales, rows, k, lead
+
+    @classmethod
+    def _made(cls, codes: torch.Tensor, scales: torch.Tensor, rows: int, k: int, lead) -> "MxTensor":
+        """Buffers that this package allocated for [rows, k]: nothing to check."""
+        t = cls.__new__(cls)
+        t.codes, t.scales, t.rows, t.k, t.lead = codes, scales, rows, k, tuple(lead)
+        return t
 
     @classmethod
     def empty(cls, rows: int, k: int, device, lead=None) -> "MxTensor":
-        row_tiles, pitch, tiles = -(-rows // 128), -(-k // BLOCK) * 16, -(-k // 256) * 2
-        return cls(torch.empty((rows, pitch), dtype=torch.uint8, device=device),
-                   torch.empty((row_tiles * tiles * 512,), dtype=torch.uint8, device=device), rows, k, lead)
+        shape, tiles = _sizes(rows, k)
+        return cls._made(torch.empty(shape, dtype=torch.uint8, device=device), torch.empty((tiles,), dtype=torch.uint8, device=device), rows, k,
+                         (rows,) if lead is None else lead)
 
     @classmethod
     def from_packed(cls, codes: torch.Tensor, scales: torch.Tensor, k: Optional[int] = None) -> "MxTensor":
@@ -108,7 +136,7 @@ def mx_quantize(x: torch.Tensor) -> MxTensor:
     if made is not None:
         codes, scales = _checked(made)
         lead = x.shape[:-1]
-        return MxTensor(codes, scales, codes.shape[0], x.shape[-1], lead)
+        return MxTensor._made(codes, scales, codes.shape[0], x.shape[-1], lead)
     device = _block.require_cuda(x, "input")
     e = _block.elem_of(x, "input")
     if x.dim() == 0 or x.shape[-1] == 0:
