@@ -136,7 +136,10 @@ def elem_of(t: torch.Tensor, what: str) -> int:
 
 
 def rows_of(t: torch.Tensor, cols: int) -> torch.Tensor:
-    """t [..., cols] as [rows, cols] with consecutive columns (a view where the strides allow)."""
+    """t [..., cols] as [rows, cols] with consecutive columns, rows that do not overlap: a view
+    where the strides allow, else (columns apart, one row expanded, a sliding window) a copy."""
     if t.dim() != 2:
         t = t.reshape(-1, cols)
-    return t if t.stride(1) == 1 or cols == 1 else t.contiguous()
+    if (t.stride(1) != 1 and cols != 1) or (t.stride(0) < cols and t.shape[0] > 1):
+        return t.contiguous()
+    return t

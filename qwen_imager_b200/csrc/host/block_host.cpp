@@ -55,7 +55,7 @@ at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, at::Device device) 
 
 void *current_stream(at::Device d) { return c10::cuda::getCurrentCUDAStream(d.index()).stream(); }
 
-// x as rows of its last dimension: false unless they are evenly spaced and their columns consecutive.
+// x as rows of its last dimension: false unless they are evenly spaced, apart, and their columns consecutive.
 struct Rows {
     int64_t rows, cols, stride;
 };
@@ -68,7 +68,7 @@ bool rows_of(const at::Tensor &x, Rows *r) {
         if (x.stride(1) != 1) return false;
         r->rows = x.size(0);
         r->stride = x.stride(0);
-        return true;
+        return r->stride >= r->cols || r->rows <= 1;
     }
     if (!x.is_contiguous()) return false;
     r->rows = x.numel() / r->cols;
