@@ -16,6 +16,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -76,15 +77,17 @@ def build_host(force: bool = False) -> str:
     base = os.path.dirname(torch.__file__)
     inc = os.path.join(base, "include")
     cuda = os.path.dirname(os.path.dirname(nvcc_path()))
-    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           "-I" + os.path.join(ROOT, "include"), "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
-           "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], HOST_SRC, "-o", HOST + ".tmp",
-           "-L" + os.path.join(base, "lib"), "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10_cuda"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("g++ failed on block_host.cpp")
-    os.replace(HOST + ".tmp", HOST)
+    with tempfile.TemporaryDirectory(dir=OUT_DIR) as work:  # this build's own: several processes may find the file stale at once
+        made = os.path.join(work, os.path.basename(HOST))
+        cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+               "-I" + os.path.join(ROOT, "include"), "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
+               "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], HOST_SRC, "-o", made,
+               "-L" + os.path.join(base, "lib"), "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10_cuda"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError("g++ failed on block_host.cpp")
+        os.replace(made, HOST)
     return HOST
 
 
@@ -95,31 +98,31 @@ def build(verbose: bool = False, force: bool = False) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
     nvcc = nvcc_path()
 
-    def compile_one(src: str):
-        obj = os.path.join(OUT_DIR, os.path.basename(src)[:-3] + ".o")
-        cmd = [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, "-c", src, "-o", obj]
-        if verbose:
-            cmd += ["-Xptxas", "-v"]
-        return src, obj, subprocess.run(cmd, capture_output=True, text=True)
+    with tempfile.TemporaryDirectory(dir=OUT_DIR) as work:  # this build's own, as above
 
-    objs = []
-    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
-        results = list(pool.map(compile_one, sources()))
-    for src, obj, res in results:
-        if verbose or res.returncode != 0:
-            sys.stderr.write(res.stdout + res.stderr)
+        def compile_one(src: str):
+            obj = os.path.join(work, os.path.basename(src)[:-3] + ".o")
+            cmd = [nvcc, *ARCH_FLAGS, *NVCC_FLAGS, "-c", src, "-o", obj]
+            if verbose:
+                cmd += ["-Xptxas", "-v"]
+            return src, obj, subprocess.run(cmd, capture_output=True, text=True)
+
+        objs = []
+        with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+            results = list(pool.map(compile_one, sources()))
+        for src, obj, res in results:
+            if verbose or res.returncode != 0:
+                sys.stderr.write(res.stdout + res.stderr)
+            if res.returncode != 0:
+                raise RuntimeError(f"nvcc failed on {os.path.basename(src)}")
+            objs.append(obj)
+        made = os.path.join(work, os.path.basename(LIB))
+        cmd = [nvcc, *ARCH_FLAGS, "-shared", "-o", made, *objs, "-Xcompiler", "-fPIC"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
-            raise RuntimeError(f"nvcc failed on {os.path.basename(src)}")
-        objs.append(obj)
-    tmp = LIB + ".tmp"
-    cmd = [nvcc, *ARCH_FLAGS, "-shared", "-o", tmp, *objs, "-Xcompiler", "-fPIC"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-        raise RuntimeError("nvcc link of libqmm.so failed")
-    os.replace(tmp, LIB)
-    for obj in objs:
-        os.remove(obj)
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError("nvcc link of libqmm.so failed")
+        os.replace(made, LIB)
     return LIB
 
 
