@@ -10,6 +10,7 @@ import ctypes
 import importlib.util
 import os
 import struct
+import warnings
 
 import torch
 
@@ -71,22 +72,34 @@ def load() -> ctypes.CDLL:
     return _lib_block
 
 
+class _General:
+    """Stands in for the extension where it cannot be had: every call goes its general way."""
+
+    mx_quantize = mx_dequantize = mx_linear = qk_norm_rotary = gated_norm = staticmethod(lambda *args: None)
+
+
 def host():
     """The extension with the operators' ordinary calls (csrc/host/block_host.cpp),
     built first when stale: a small operator's time is the time of its call
-    (B200, one-token linear: 14 us through the checks here and ctypes)."""
+    (B200, one-token linear: 14 us through the checks here and ctypes).  It only saves
+    time: where it cannot be built, a warning says so and the operators run without."""
     global _host_module
     if _host_module is None:
         lib = load()
-        if _build.host_is_stale():
-            try:
-                _build.build_host()
-            except Exception as exc:  # no compiler, or an error: the built one, if any, still serves
-                if not os.path.exists(_build.HOST):
-                    raise QmmError(_lib.QMM_ERR_CUDA, f"_qmm_host.so is not built and cannot be built: {exc}")
-        spec = importlib.util.spec_from_file_location("_qmm_host", _build.HOST)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
+        try:
+            if _build.host_is_stale():
+                try:
+                    _build.build_host()
+                except Exception:  # no compiler, or an error: the built one, if any, still serves
+                    if not os.path.exists(_build.HOST):
+                        raise
+            spec = importlib.util.spec_from_file_location("_qmm_host", _build.HOST)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except Exception as exc:
+            warnings.warn(f"_qmm_host.so cannot be used, calls of the block operators take longer: {exc}", RuntimeWarning, stacklevel=3)
+            _host_module = _General
+            return _host_module
         module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "qmm_mx4_linear", "qmm_mx4_linear_workspace_bytes", "qmm_mx4_quantize", "qmm_mx4_dequantize", "qmm_qk_norm_rotary",
             "qmm_gated_residual_norm")))
