@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
-import os
 import struct
 import warnings
 
@@ -87,12 +86,8 @@ def host():
     if _host_module is None:
         lib = load()
         try:
-            if _build.host_is_stale():
-                try:
-                    _build.build_host()
-                except Exception:  # no compiler, or an error: the built one, if any, still serves
-                    if not os.path.exists(_build.HOST):
-                        raise
+            if _build.host_is_stale():  # (never loaded stale: it fills the structs of the headers that it was built from)
+                _build.build_host()
             spec = importlib.util.spec_from_file_location("_qmm_host", _build.HOST)
             module = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(module)

@@ -11,6 +11,7 @@ Usage: python -m qwen_imager_b200.build [--verbose]
 from __future__ import annotations
 
 import glob
+import hashlib
 import os
 import shutil
 import subprocess
@@ -62,8 +63,26 @@ def is_stale() -> bool:
     return _older(LIB, sources() + headers() + [__file__])
 
 
+def host_key() -> str:
+    """What the extension is built from and for: its sources, this file, and the torch and
+    Python whose binary interfaces it uses.  Compiled into it (`key`)."""
+    import torch
+
+    h = hashlib.sha256()
+    for path in (HOST_SRC, os.path.join(ROOT, "include", "qmm_block.h"), os.path.join(ROOT, "include", "qmm.h"), __file__):
+        with open(path, "rb") as f:
+            h.update(f.read())
+    h.update(f"{torch.__version__} {sys.implementation.cache_tag}".encode())
+    return h.hexdigest()
+
+
 def host_is_stale() -> bool:
-    return _older(HOST, [HOST_SRC, os.path.join(ROOT, "include", "qmm_block.h"), os.path.join(ROOT, "include", "qmm.h"), __file__])
+    """Whether the extension is missing or does not hold the present key (times of files say
+    nothing about the torch that it was built for)."""
+    if not os.path.exists(HOST):
+        return True
+    with open(HOST, "rb") as f:
+        return host_key().encode() not in f.read()
 
 
 def build_host(force: bool = False) -> str:
@@ -81,7 +100,7 @@ def build_host(force: bool = False) -> str:
         made = os.path.join(work, os.path.basename(HOST))
         cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
                "-I" + os.path.join(ROOT, "include"), "-I" + inc, "-I" + os.path.join(inc, "torch", "csrc", "api", "include"),
-               "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], HOST_SRC, "-o", made,
+               "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], f'-DQMM_HOST_KEY="{host_key()}"', HOST_SRC, "-o", made,
                "-L" + os.path.join(base, "lib"), "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10_cuda"]
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:

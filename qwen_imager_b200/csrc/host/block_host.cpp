@@ -370,4 +370,16 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_qmm_host", nullptr, -1, methods, 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__qmm_host(void) { return PyModule_Create(&module); }
+// What this file was built from and for; the package loads no other (build.py).
+#ifndef QMM_HOST_KEY
+#define QMM_HOST_KEY ""
+#endif
+
+PyMODINIT_FUNC PyInit__qmm_host(void) {
+    PyObject *m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "key", QMM_HOST_KEY) != 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}
