@@ -63,7 +63,8 @@ QMM_API qmm_status qmm_mx4_quantize(const void *x, int32_t elem, int64_t rows, i
                                     uint8_t *codes, uint8_t *scales, void *stream);
 
 /* dst [rows, k] (row-major, contiguous; bf16, f32 or f16) = the values of `w`.
- * bf16 and f32 hold every value exactly; f16 rounds (past 65504: infinity). */
+ * bf16 and f32 hold every value below 2^128 exactly (scales 253 and 254 reach
+ * past it: infinity); f16 rounds (past 65504: infinity). */
 QMM_API qmm_status qmm_mx4_dequantize(const qmm_mx4 *w, void *dst, int32_t elem, void *stream);
 
 /* Scales between row-major order (uint8 [rows, ceil(k / 32)], as checkpoints

@@ -2,7 +2,7 @@
 // allocation and the C entry point (include/qmm_block.h).
 //
 // A small operator's time is the time of its call: on B200 a one-token linear
-// (7.7 us on the device) took 14 us through the Python checks and ctypes.  Each function
+// (7.1 us on the device) took 14 us through the Python checks and ctypes.  Each function
 // here takes exactly the operands that need no conversion and returns its outputs;
 // for anything else (another type, device or layout, an argument error) it returns
 // None, and the Python function goes its general way, which converts or raises.  A

@@ -860,9 +860,6 @@ static qmm_status launch_gemm_pair(const qmm_mx4 &w, const qmm_mx4 &x, const qmm
     return e == cudaSuccess ? QMM_OK : cuda_fail(e, "mxfp4 gemm launch");
 }
 
-// Few tokens or few tiles: the kernel that splits k.  Pairs where their 256 x 256
-// tiles fill at least half of the SM pairs; below that the 128 x 192 tiles keep more
-// SMs busy.
 // Whether pairs of CTAs take the product in less time: turns of tiles over the device,
 // each as long as its products, 2.0 ns a column of k with either tile, or, where k is
 // short, its epilogue: 4.3 us (7 with an activation) for a CTA of a pair, 1.7 (2.9) for

@@ -44,9 +44,10 @@ __device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint64_t a, uint64_t b, 
 }
 
 // t * sigmoid(z) of two values: both activations in one exponential and one
-// reciprocal a value (GELU's 0.5 (1 + tanh u) is sigmoid(2 u)).  The fast forms are
-// good to a few 2^-22 of the result, far below its rounding to bf16; past their range
-// they give 0 or t.
+// reciprocal a value (GELU's 0.5 (1 + tanh u) is sigmoid(2 u)).  Beside a few 2^-22 of
+// the fast forms, the rounding of the exponent y = -z log2(e) costs about |y| 2^-23 of
+// the result where t is negative: 2^-16 at the most, as past |y| = 126 (results below
+// 1e-36) it is 0; the rounding to bf16 is 2^-8.  Past their range the forms give 0 or t.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

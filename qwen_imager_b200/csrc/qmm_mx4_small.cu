@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto copy_x = [&](int i) {
             const int s = i % S;
             tma_load_2d(smem + C::kBOff + s * C::kBBytes, &tmap_x, &full[s], (kb0 + i) * kRowBytes, m0);
-            // rows m0 .. m0 + NT of a 128-row scale tile start at byte 4 (m0 % 128 / 32) of its cells: the MMA's scale address says so
+            // (m0 is a multiple of 128: tiles of fewer tokens come alone)
             bulk_load(smem + C::kSfbOff + s * C::kSfBytes, p.x_scales + ((int64_t)(m0 >> 7) * p.sf_tiles + (kb0 + i) * 2) * kSfTile,
                       C::kSfBytes, &full[s]);
         };
@@ -191,7 +191,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ------------------------------------------------------------ MMA issuer
         const uint64_t adesc0 = sdesc_kmajor_sw128(smem_u32(smem + C::kAOff)), bdesc0 = sdesc_kmajor_sw128(smem_u32(smem + C::kBOff));
         const uint64_t sadesc0 = sdesc_scales(smem_u32(smem + C::kSfaOff)), sbdesc0 = sdesc_scales(smem_u32(smem + C::kSfbOff));
-        const uint32_t shift = quantise ? 0 : (uint32_t)(m0 & 127) >> 5;
         uint32_t acc = 0;
         int i = 0;
         for (; i < nkb; ++i) {
@@ -213,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {
                     tc_mma_mxf4(tmem, ad + kk * 2, bd + kk * 2, C::kIdesc | idesc_scale_id((kk & 1) * 2), sfa + (kk >> 1) * 4,
-                                sfb + (kk >> 1) * 4 + shift, acc);
+                                sfb + (kk >> 1) * 4, acc);
                     acc = 1;
                 }
                 tc_commit(&empty[s]);

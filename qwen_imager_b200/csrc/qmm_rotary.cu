@@ -274,7 +274,9 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qm
 }
 
 // Any dim up to 256, any pairs, any alignment: lane l takes pairs l, l + 32, ...
-// and the unrotated columns likewise, element by element.
+// and the unrotated columns likewise, element by element, one head at a time.  Bound by
+// its narrow accesses (B200, 16896 x 48 x 128 bf16 in halves with 31 pairs 315 us, 0.20 of
+// the measured HBM rate).
 template <typename T>
 __global__ void __launch_bounds__(kWarps * 32) rotary_any_kernel(const qmm_rotary_args a, const int heads_per_warp) {
     const int lane = threadIdx.x & 31;

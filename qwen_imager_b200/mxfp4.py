@@ -6,8 +6,9 @@
 
 Beside the MLX affine `Linear`, whose weights are dequantised for bf16 products,
 `MxLinear` quantises the activations too and multiplies codes on the tensor
-cores' block-scaled 4-bit path.  Its `forward_fused` takes the arguments of
-`Linear.forward_fused`, so callers of the one run with the other.  Forward only.
+cores' block-scaled 4-bit path.  Its `forward_fused` takes the epilogue's
+arguments of `Linear.forward_fused` (gate, residual, activation, out, bias,
+residual_mul), so callers that pass these run with either.  Forward only.
 """
 from __future__ import annotations
 
@@ -111,7 +112,7 @@ class MxTensor:
         return out
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-        """The values, [..., k]; exact in bf16 and f32."""
+        """The values, [..., k]; exact in bf16 and f32 (below 2^128)."""
         if dtype is torch.bfloat16 and len(self.lead) == 1:
             out = _host().mx_dequantize(self.codes, self.scales, self.rows, self.k)
             if out is not None:
