@@ -106,8 +106,9 @@ __device__ __forceinline__ void runs_to_pairs(const Runs<T> &r, float2 (&a)[2], 
         }
     }
 }
+// The inverse, word for word.
 template <typename T, Layout L>
-__device__ __forceinline__ void store_pairs(T *p, int ca, int cb, const float2 (&a)[2], const float2 (&b)[2]) {
+__device__ __forceinline__ Runs<T> pairs_to_runs(const float2 (&a)[2], const float2 (&b)[2]) {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -119,14 +120,26 @@ __device__ __forceinline__ void store_pairs(T *p, int ca, int cb, const float2 (
             v[4 * i + 1] = b[i].x, v[4 * i + 3] = b[i].y;
         }
     }
+    Runs<T> r;
     if constexpr (sizeof(T) == 4) {
-        *reinterpret_cast<float4 *>(p + ca) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4 *>(p + cb) = make_float4(v[4], v[5], v[6], v[7]);
-    } else if constexpr (L == kWide) {
-        *reinterpret_cast<uint4 *>(p + ca) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.w[i] = __float_as_uint(v[i]);
     } else {
-        *reinterpret_cast<uint2 *>(p + ca) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-        *reinterpret_cast<uint2 *>(p + cb) = make_uint2(pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    }
+    return r;
+}
+template <typename T, Layout L>
+__device__ __forceinline__ void store_runs(T *p, int ca, int cb, const Runs<T> &r) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<uint4 *>(p + ca) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+        *reinterpret_cast<uint4 *>(p + cb) = make_uint4(r.w[4], r.w[5], r.w[6], r.w[7]);
+    } else if constexpr (L == kWide) {
+        *reinterpret_cast<uint4 *>(p + ca) = make_uint4(r.w[0], r.w[1], r.w[2], r.w[3]);
+    } else {
+        *reinterpret_cast<uint2 *>(p + ca) = make_uint2(r.w[0], r.w[1]);
+        *reinterpret_cast<uint2 *>(p + cb) = make_uint2(r.w[2], r.w[3]);
     }
 }
 
@@ -143,9 +156,10 @@ struct Heads {
 // halves pairs % 4 == 0, heads aligned as the layout says.  NORM: some weight is
 // given; POW2: dim / 8 is a power of two; TAIL: some columns are not turned.  A turn by 0
 // would mix an infinity or NaN of one into its lane's neighbour (0 times either is NaN),
-// so selects keep them apart (B200, 16896 x 48 x 128 with 32 of 64 pairs 71.6 -> 75.8 us, in
-// halves 77.8 -> 80.7; 2 x 14317 x 24 x 72 f16 41.0 -> 43.0; a branch on the head's sum of
-// squares and predicated products cost registers and as much time).
+// so without a norm their words leave as they came, and with one selects keep them apart
+// (B200, 2 x 14317 x 24 x 72 f16 41.0 -> 42.5 us; with a norm, 16896 x 48 x 128 with 32 of
+// 64 pairs 71.6 -> 75.8, in halves 77.8 -> 80.7; a branch on the head's sum of squares and
+// predicated products cost registers and as much time).
 template <typename T, Layout L, bool NORM, bool POW2, bool TAIL, int kTurns>
 __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qmm_rotary_args a, const int heads_per_warp) {
     constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;  // heads a lane group has in flight
@@ -209,8 +223,8 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qm
                     fb[i] = mul_f32x2(wo[i], make_float2(-sn[i].x, -sn[i].y));
                     fc[i] = mul_f32x2(we[i], sn[i]);
                     fd[i] = mul_f32x2(wo[i], cs[i]);
-                    if (TAIL && !turns(2 * i)) fb[i].x = fc[i].x = -0.0f;  // 0 * -0 changes no number that it is added to
-                    if (TAIL && !turns(2 * i + 1)) fb[i].y = fc[i].y = -0.0f;
+                    if (TAIL && NORM && !turns(2 * i)) fb[i].x = fc[i].x = -0.0f;  // 0 * -0 changes no number that it is added to
+                    if (TAIL && NORM && !turns(2 * i + 1)) fb[i].y = fc[i].y = -0.0f;
                 }
             }
 #pragma unroll
@@ -247,7 +261,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qm
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         float2 xc = x[q], yc = y[q];
-                        if constexpr (TAIL) {
+                        if constexpr (TAIL && NORM) {
                             const bool first = turns(2 * q), second = turns(2 * q + 1);
                             xc = make_float2(first ? xc.x : 0.0f, second ? xc.y : 0.0f);
                             yc = make_float2(first ? yc.x : 0.0f, second ? yc.y : 0.0f);
@@ -255,7 +269,12 @@ __global__ void __launch_bounds__(kWarps * 32, kResident) rotary_kernel(const qm
                         oa[q] = fma_f32x2(x[q], fa[q], mul_f32x2(yc, fb[q]));
                         ob[q] = fma_f32x2(xc, fc[q], mul_f32x2(y[q], fd[q]));
                     }
-                    store_pairs<T, L>(dst + j * dst_step, ca, cb, oa, ob);
+                    Runs<T> out = pairs_to_runs<T, L>(oa, ob);
+                    if constexpr (TAIL && !NORM) {
+#pragma unroll
+                        for (int i = 0; i < (int)sizeof(T) * 2; ++i) out.w[i] = turns(i * 2 / (int)sizeof(T)) ? out.w[i] : raw[j].w[i];
+                    }
+                    store_runs<T, L>(dst + j * dst_step, ca, cb, out);
                 }
             }
             src += src_step * kAhead;
