@@ -506,7 +506,9 @@ __global__ void __launch_bounds__(Cfg<TN>::kThreads, 1)
 // work, and spreads six scale copies over it.  B200, back to back: 4352 x 12288 ->
 // 3072 57 us (5.8 PFLOP/s; one-CTA tiles 77), 16384 x 3072 -> 12288 257 us, with GELU
 // 277 (309, 332), without the epilogue's work 220: operands out of L2 and the power
-// that all of it costs bound it.  16 epilogue warps of 96 registers took 291 with GELU.
+// that all of it costs bound it (59, 265 and 289 in bursts of 100 launches on another
+// card; after half a second the power cap leaves 1.6 GHz, 66, 295 and 323).  16 epilogue
+// warps of 96 registers took 291 with GELU.
 //
 // Two accumulators of 256 columns and a scale slot for each stage do not fit the
 // 512 columns of tensor memory, so the accumulators share 96 columns, [0, 256) and

@@ -22,8 +22,8 @@ namespace qmm {
 namespace rotary {
 
 constexpr int kWarps = 4;
-// CTAs an SM: 32 warps cover the loads (B200, 16896 x 48 heads x 128 bf16: 70 us, 0.90 of
-// the measured HBM rate; before lanes shared their sines 73, with 16 warps 95, with 40 79).
+// CTAs an SM: 32 warps cover the loads (B200, 16896 x 48 heads x 128 bf16: 72 us, 0.88 of
+// the measured HBM rate, 70 where operands stay the same; before lanes shared their sines 73, with 16 warps 95, with 40 79).
 constexpr int kResident = 8;
 
 // A position as two terms: whole numbers past 2^24 do not fit one.
